@@ -26,6 +26,8 @@ DEVERR_BITS = {
     1 << 2: "tensor-core completion was never signalled",
     1 << 3: "copies in flight never landed while aborting",
     1 << 4: "a peer rank never released a gathered-output slot",
+    1 << 5: "a page index or sequence offset was out of range, taken twice or of a free page",
+    1 << 6: "no free page was left to hand out",
 }
 
 # Every function the header declares (checked by the CPU test suite).
@@ -48,7 +50,17 @@ EXPORTED = (
     "gdn_gather_wait",
     "gdn_gather_wait_counter",
     "gdn_state_affine",
+    "lin_decode_launch",
+    "lin_prefill_launch",
+    "lin_prefill_workspace_size",
+    "pages_workspace_size",
+    "pages_copy_launch",
+    "pages_fork_launch",
+    "pages_free_launch",
+    "pages_compact_launch",
 )
+PAGES_MAX_POOLS = 64
+PAGES_MAX_PAGES = 1 << 19
 IPC_HANDLE_BYTES = 64
 
 
@@ -120,6 +132,53 @@ class PrefillArgs(ctypes.Structure):
     ]
 
 
+def _fields(*groups):
+    """(type, "name name ...") groups as a ctypes field list."""
+    return [(name, typ) for typ, names in groups for name in names.split()]
+
+
+_vp, _i32, _i64 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64
+
+
+class LinDecodeArgs(ctypes.Structure):
+    _fields_ = _fields(
+        (_vp, "q k v g state_in state_out o index"),
+        (_i64, "q_sb q_sh k_sb k_sh v_sb v_sh o_sb o_sh g_sb g_sh state_in_sp state_out_sp"),
+        (_i32, "B Hqk Hv dk dv pages io_dtype g_dtype gate_kind"),
+        (ctypes.c_float, "scale"),
+        (_vp, "status"),
+    )
+
+
+class LinPrefillArgs(ctypes.Structure):
+    _fields_ = _fields(
+        (_vp, "q k v g initial_state final_state o cu_seqlens index"),
+        (_i64, "q_sb q_st q_sh k_sb k_st k_sh v_sb v_st v_sh o_sb o_st o_sh g_sb g_st g_sh "
+               "initial_sp final_sp"),
+        (_i32, "B T Hqk Hv dk dv pages io_dtype g_dtype"),
+        (ctypes.c_float, "scale"),
+        (_vp, "workspace"),
+        (ctypes.c_size_t, "workspace_bytes"),
+        (_vp, "status"),
+    )
+
+
+class PagesPool(ctypes.Structure):
+    _fields_ = _fields((_vp, "base"), (_i64, "page_stride page_bytes"))
+
+
+class PagesArgs(ctypes.Structure):
+    _fields_ = _fields(
+        (ctypes.POINTER(PagesPool), "pools"),
+        (_i32, "n_pools pages"),
+        (_vp, "used used_out"),
+        (_i32, "n"),
+        (_vp, "src dst remap count workspace"),
+        (ctypes.c_size_t, "workspace_bytes"),
+        (_vp, "status"),
+    )
+
+
 _lock = threading.Lock()
 _lib = None
 
@@ -171,6 +230,18 @@ def load(path: str | Path | None = None):
         L.gdn_gather_wait_counter.restype = ctypes.c_int
         L.gdn_state_affine.argtypes = [vp, vp, vp, vp, i32, i32, vp]
         L.gdn_state_affine.restype = ctypes.c_int
+        L.lin_decode_launch.argtypes = [ctypes.POINTER(LinDecodeArgs), vp]
+        L.lin_prefill_launch.argtypes = [ctypes.POINTER(LinPrefillArgs), vp]
+        L.lin_prefill_workspace_size.argtypes = [ctypes.POINTER(LinPrefillArgs)]
+        L.pages_workspace_size.argtypes = [ctypes.POINTER(PagesArgs)]
+        for fn in (L.lin_prefill_workspace_size, L.pages_workspace_size):
+            fn.restype = ctypes.c_size_t
+        for fn in (L.pages_copy_launch, L.pages_fork_launch, L.pages_free_launch,
+                   L.pages_compact_launch):
+            fn.argtypes = [ctypes.POINTER(PagesArgs), vp]
+            fn.restype = ctypes.c_int
+        for fn in (L.lin_decode_launch, L.lin_prefill_launch):
+            fn.restype = ctypes.c_int
         for fn in (L.gdn_ipc_handle, L.gdn_ipc_open, L.gdn_ipc_close, L.gdn_gather_push,
                    L.gdn_gather_wait):
             fn.restype = ctypes.c_int

@@ -1,8 +1,9 @@
 /*
  * gdn_b200.h — C ABI of the B200 (sm_100a) gated delta-rule library.
  *
- * The library implements three operations of the gated delta rule
- * (GDN / KDA linear attention), each as hand-written sm_100a CUDA:
+ * The library implements the operations of the gated delta rule
+ * (GDN / KDA linear attention), linear attention with a plain decay per head,
+ * and the pages of a cache of their states, as hand-written sm_100a CUDA:
  *
  *   GDN decode (one token per sequence, scalar gate per head)
  *       S      <- a * S                      a = exp(g) (log gate) or g (linear gate)
@@ -85,6 +86,9 @@ enum {
   GDN_DEVERR_MMA_TIMEOUT = 1u << 2,   /* tensor-core completion never signalled   */
   GDN_DEVERR_DRAIN_TIMEOUT = 1u << 3, /* copies in flight never landed on abort   */
   GDN_DEVERR_PEER_TIMEOUT = 1u << 4,  /* a peer never released an output slot     */
+  GDN_DEVERR_BAD_INDEX = 1u << 5,     /* a page index or sequence offset was out  */
+                                      /* of range, taken twice or of a free page  */
+  GDN_DEVERR_POOL_FULL = 1u << 6,     /* no free page was left to hand out        */
 };
 
 /*
@@ -352,6 +356,154 @@ int gdn_state_affine(const float* M, const float* L, const float* S_in, float* S
  * arrival counter of the fused output all-gather (gdn_peer_out_t.arrive). */
 int gdn_gather_wait_counter(const uint32_t* counter, uint32_t target, uint32_t* status,
                             gdn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Linear attention with a decay for each head (no delta rule):
+ *
+ *     S_t = a_t S_{t-1} + k_t v_t^T        o_t = scale * S_t^T q_t
+ *
+ * with a_t = exp(g_t) a scalar per value head, data-dependent (g per token)
+ * or fixed (one g per head; strides of 0 over batch and time).  Heads, the
+ * state layout and q/k head sharing are those of the gated delta rule.  The
+ * reference has no such operator; layers of this kind alternate with GDN
+ * layers in hybrid models and keep the same states.
+ *
+ * States may live in a pool of pages [P, Hv, d_k, d_v], one page per sequence
+ * (page p at state + p * state_sp elements; contiguous inside).  With `index`
+ * (int32, device) row b uses page index[b]; without it, page b.  A negative
+ * index is a row without a page.  An index >= P, or one that an earlier row
+ * of the call holds, sets GDN_DEVERR_BAD_INDEX and is treated as negative.
+ * ---------------------------------------------------------------------- */
+
+/*
+ * One token per sequence.  A row without a page gets a zero output row and
+ * touches no state.  Strides are in ELEMENTS; rows of q/k/v/o are contiguous,
+ * their bases and strides 16-byte aligned, as are the states (state_sp a
+ * multiple of 4).  state_out may equal state_in (in place) or be disjoint
+ * from it; the pages of idle rows are not copied to a disjoint state_out.
+ * d_k in {64, 128, 256}, d_v a multiple of 64.
+ */
+typedef struct {
+  const void* q;         /* [B, Hqk, d_k]  io_dtype                          */
+  const void* k;         /* [B, Hqk, d_k]  io_dtype                          */
+  const void* v;         /* [B, Hv,  d_v]  io_dtype                          */
+  const void* g;         /* [B, Hv] or, with g_sb = 0, [Hv]   g_dtype        */
+  const float* state_in; /* P pages of [Hv, d_k, d_v] fp32                   */
+  float* state_out;      /* same layout; may equal state_in                  */
+  void* o;               /* [B, Hv, d_v]   io_dtype                          */
+  const int32_t* index;  /* [B] page of each row, or NULL (page b; P >= B)   */
+  int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, o_sb, o_sh;
+  int64_t g_sb, g_sh;
+  int64_t state_in_sp, state_out_sp; /* elements between pages               */
+  int32_t B, Hqk, Hv, dk, dv, pages;
+  int32_t io_dtype;      /* GDN_DT_BF16 or GDN_DT_F16                        */
+  int32_t g_dtype;       /* any GDN_DT_*                                     */
+  int32_t gate_kind;     /* GDN_GATE_LOG or GDN_GATE_LINEAR                  */
+  float scale;
+  uint32_t* status;      /* optional device word for GDN_DEVERR_* bits       */
+} lin_decode_args_t;
+
+int lin_decode_launch(const lin_decode_args_t* args, gdn_stream_t stream);
+
+/*
+ * T tokens per sequence: the same recurrence in chunks.  Dense form
+ * (cu_seqlens NULL): B sequences of T tokens.  Packed form: B sequences laid
+ * end to end over T rows, sequence n being rows cu_seqlens[n] ..
+ * cu_seqlens[n+1] - 1 (int32, device; empty sequences allowed); the batch
+ * strides are then not used, rows outside every sequence are left as they
+ * were, and a sequence whose offsets do not lie in 0 <= start <= end <= T
+ * sets GDN_DEVERR_BAD_INDEX and is left out.  Sequence n starts from page
+ * index[n] (or n) of initial_state (NULL: from zero) and leaves its final
+ * state in the same page of final_state, which may equal initial_state or be
+ * disjoint from it.  A sequence with a negative index starts from zero and
+ * its state is not kept; one of no tokens keeps its initial state.
+ * d_k in {64, 128}, d_v a multiple of 64.  Strides as for the decode step.
+ * Log gates only.  Workspace: lin_prefill_workspace_size(args) bytes (0 for
+ * many shapes), 16-byte aligned, owned by the caller.
+ */
+typedef struct {
+  const void* q;              /* [B, T, Hqk, d_k] or packed [T, Hqk, d_k]    */
+  const void* k;
+  const void* v;              /* [B, T, Hv, d_v] or packed [T, Hv, d_v]      */
+  const void* g;              /* [B, T, Hv], packed [T, Hv], or [Hv] (g_st = 0) */
+  const float* initial_state; /* pages of [Hv, d_k, d_v] fp32, or NULL       */
+  float* final_state;         /* pages of [Hv, d_k, d_v] fp32                */
+  void* o;                    /* as v                                        */
+  const int32_t* cu_seqlens;  /* [B + 1], or NULL                            */
+  const int32_t* index;       /* [B], or NULL                                */
+  int64_t q_sb, q_st, q_sh, k_sb, k_st, k_sh, v_sb, v_st, v_sh, o_sb, o_st, o_sh;
+  int64_t g_sb, g_st, g_sh;
+  int64_t initial_sp, final_sp; /* elements between pages                    */
+  int32_t B, T, Hqk, Hv, dk, dv, pages;
+  int32_t io_dtype, g_dtype;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+  uint32_t* status;
+} lin_prefill_args_t;
+
+size_t lin_prefill_workspace_size(const lin_prefill_args_t* args);
+int lin_prefill_launch(const lin_prefill_args_t* args, gdn_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Pages of a cache of recurrent states: one page per sequence, in one or
+ * several pools of the same page count (one per layer, say; page sizes may
+ * differ).  `used` holds one int32 per page, 0 = free.  Nothing is decided on
+ * the host, so every call can be captured in a graph.  Pages are handed out
+ * lowest first.  No counterpart in the reference.
+ * ---------------------------------------------------------------------- */
+#define PAGES_MAX_POOLS 64
+#define PAGES_MAX_PAGES (1 << 19)
+
+typedef struct {
+  void* base;          /* page p is page_bytes bytes at base + p * page_stride */
+  int64_t page_stride; /* bytes, a multiple of 16                             */
+  int64_t page_bytes;  /* a multiple of 16                                    */
+} pages_pool_t;
+
+typedef struct {
+  const pages_pool_t* pools; /* HOST array of n_pools entries                 */
+  int32_t n_pools;           /* 0 .. PAGES_MAX_POOLS                          */
+  int32_t pages;             /* pages in every pool                           */
+  const int32_t* used;       /* [pages]                                       */
+  int32_t* used_out;         /* [pages]; may equal used                       */
+  int32_t n;                 /* entries of src / dst / index                  */
+  const int32_t* src;        /* see the calls                                 */
+  int32_t* dst;
+  int32_t* remap;            /* [pages], pages_compact_launch                 */
+  int32_t* count;            /* [1], pages_compact_launch                     */
+  int32_t* workspace;        /* pages_workspace_size(args) bytes              */
+  size_t workspace_bytes;
+  uint32_t* status;
+} pages_args_t;
+
+size_t pages_workspace_size(const pages_args_t* args);
+
+/* Page src[i] -> page dst[i] of every pool, i < n.  Entries with a negative
+ * src or dst are skipped.  An entry is also skipped, with
+ * GDN_DEVERR_BAD_INDEX, when an index is out of range, when another entry has
+ * the same destination, or when its destination is some entry's source; so
+ * what is copied does not depend on the order of the copies.  dst is read. */
+int pages_copy_launch(const pages_args_t* args, gdn_stream_t stream);
+
+/* dst[i] = the next free page, holding a copy of page src[i], i < n; the same
+ * source may be given many times.  src NULL: the pages are handed out as they
+ * are (pools unused).  dst[i] = -1 where src[i] is negative; likewise, with
+ * GDN_DEVERR_BAD_INDEX, where src[i] is out of range or free, and with
+ * GDN_DEVERR_POOL_FULL when no free page is left. */
+int pages_fork_launch(const pages_args_t* args, gdn_stream_t stream);
+
+/* Marks pages src[i] free.  Negative entries are skipped; one out of range, or
+ * already free, sets GDN_DEVERR_BAD_INDEX. */
+int pages_free_launch(const pages_args_t* args, gdn_stream_t stream);
+
+/* Moves the used pages behind the first `count` places (count = number of used
+ * pages) into the free ones among them, both in ascending order, so that the
+ * used pages become pages 0 .. count - 1.  remap[p] = where page p now is, -1
+ * for a free page.  With n > 0, dst[i] = remap[src[i]] (src may equal dst):
+ * -1 for a negative src[i] and, with GDN_DEVERR_BAD_INDEX, for one out of
+ * range or free.  Pages behind the first `count` keep their bytes. */
+int pages_compact_launch(const pages_args_t* args, gdn_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,345 @@
+"""Linear attention with a decay per head on the GPU, against its definition in
+64 bits.
+
+Tolerances, from the arithmetic (u = half a step of the I/O type, w = 2^-8 of
+bf16, e = 2^-24 of fp32; `abs` the sum of the terms' absolute values):
+
+* decode keeps everything in fp32: a state element has the gate's exp (a few
+  units, growing with |g| through the product with log2 e) and two roundings; an
+  output adds the d_k products and one rounding to the I/O type.
+* prefill rounds the decayed scores to the I/O type (u), the scaled queries and
+  the states they meet to bf16 (2 w), and the output (u).  The states' updates
+  split the decayed values into two parts of the I/O type: what is left is
+  u^2 of each term, and in f16 half a step of its smallest number.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from lin_oracle import half_step, steps
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E = 2.0 ** -24
+W = half_step(torch.bfloat16)
+
+
+def make(lead, Hqk, Hv, dk, dv, io, seed, gmin=-0.2, g_dtype=torch.float32, gate="token"):
+    gen = torch.Generator().manual_seed(seed)
+    q = torch.randn(*lead, Hqk, dk, generator=gen).to(io)
+    k = torch.randn(*lead, Hqk, dk, generator=gen).to(io)
+    v = torch.randn(*lead, Hv, dv, generator=gen).to(io)
+    g = (torch.rand(*(lead if gate == "token" else ()), Hv, generator=gen) * gmin).to(g_dtype)
+    return q, k, v, g
+
+
+def check_prefill(o, S, ref, io, k, v):
+    ro, rS, oa, Sa = ref
+    u = half_step(io)
+    tol = u * ro.abs() + (u + 2 * W + 64 * E) * oa + 1e-12
+    assert bool(((o.double() - ro).abs() <= tol).all()), float(((o.double() - ro).abs() / tol).max())
+    tiny = 2.0 ** -25 if io == torch.float16 else 0.0
+    tolS = (u * u + 64 * E) * Sa + tiny * k.double().abs().sum(0).amax() + 1e-12
+    assert bool(((S.double() - rS).abs() <= tolS).all()), float(((S.double() - rS).abs() / tolS).max())
+
+
+# ------------------------------------------------------------------ decode
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 192), (128, 64), (128, 128), (256, 64), (256, 128)])
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,Hqk,Hv", [(1, 1, 1), (3, 2, 4), (37, 3, 3)])
+def test_decode(pkg, dk, dv, io, B, Hqk, Hv):
+    q, k, v, g = make((B,), Hqk, Hv, dk, dv, io, B + dk)
+    S = torch.randn(B, Hv, dk, dv, generator=torch.Generator().manual_seed(1))
+    st = S.to(DEV)
+    o = pkg.lin_decode(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), st, scale=0.5, check=True).cpu()
+    check_decode(o, st.cpu(), q, k, v, g, S, 0.5, io)
+
+
+def check_decode(o, st, q, k, v, g, S, scale, io, rows=None):
+    dk = q.shape[-1]
+    for b in rows if rows is not None else range(q.shape[0]):
+        gb = g[b : b + 1] if g.dim() == 2 else g[None]
+        ro, rS, oa, Sa = steps(q[b : b + 1], k[b : b + 1], v[b : b + 1], gb, S[b], scale)
+        c = 8 + 4 * float(gb.float().abs().max())
+        assert bool(((st[b].double() - rS).abs() <= c * E * Sa).all())
+        tol = half_step(io) * ro[0].abs() + (dk + c) * E * oa[0] + 2.0 ** -25 * (io == torch.float16)
+        assert bool(((o[b].double() - ro[0]).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("gate", ["token", "head"])
+@pytest.mark.parametrize("g_dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_decode_gates(pkg, gate, g_dtype):
+    q, k, v, g = make((5,), 2, 2, 64, 64, torch.bfloat16, 3, gmin=-3.0, g_dtype=g_dtype, gate=gate)
+    S = torch.randn(5, 2, 64, 64)
+    st = S.to(DEV)
+    args = [x.to(DEV) for x in (q, k, v, g)]
+    o = pkg.lin_decode(*args, st, check=True).cpu()
+    check_decode(o, st.cpu(), q, k, v, g, S, 1.0, torch.bfloat16)
+    lin = S.to(DEV)
+    o2 = pkg.lin_decode(*args[:3], args[3].float().exp(), lin, gate="linear", check=True).cpu()
+    torch.testing.assert_close(lin.cpu(), st.cpu(), rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(o2, o, rtol=2 * half_step(torch.bfloat16), atol=1e-3)
+
+
+def test_decode_reset_gate_forgets(pkg):
+    """g = -inf (decay 0) drops the old state whole."""
+    q, k, v, _ = make((2,), 1, 2, 64, 64, torch.bfloat16, 4)
+    g = torch.tensor([[float("-inf"), 0.0], [0.0, float("-inf")]])
+    S = torch.randn(2, 2, 64, 64)
+    st = S.to(DEV)
+    o = pkg.lin_decode(q.to(DEV), k.to(DEV), v.to(DEV), g.to(DEV), st, check=True).cpu()
+    kv = k.double()[:, :, :, None] * v.double()[:, :, None, :]
+    want = torch.where(g[:, :, None, None] < 0, 0.0, S.double()) + kv
+    assert float((st.cpu().double() - want).abs().max()) <= 4 * E * float(want.abs().max())
+    assert torch.isfinite(o).all()
+
+
+def test_decode_pages_idle_bad_and_shared_rows(pkg):
+    B, P = 9, 12
+    q, k, v, g = make((B,), 2, 4, 64, 128, torch.float16, 5)
+    pool = torch.randn(P, 4, 64, 128)
+    index = torch.tensor([3, -1, 0, 11, 3, 12, 7, -5, 2 ** 31 - 1], dtype=torch.int32)
+    good = {0: 3, 2: 0, 3: 11, 6: 7}  # row 4 wants the page of row 0; 5 and 8 lie outside
+    st = pool.to(DEV)
+    out = torch.full((B, 4, 128), float("nan"), dtype=torch.float16, device=DEV)
+    args = [x.to(DEV) for x in (q, k, v, g)]
+    with pytest.raises(pkg.GDNError, match="index"):
+        pkg.lin_decode(*args, st, index=index.to(DEV), out=out, check=True)
+    o, st = out.cpu(), st.cpu()
+    rows = sorted(good)
+    check_decode(o[rows], st[[good[r] for r in rows]], q[rows], k[rows], v[rows], g[rows],
+                 pool[[good[r] for r in rows]], 1.0, torch.float16)
+    idle = [r for r in range(B) if r not in good]
+    assert bool((o[idle] == 0).all())
+    rest = [p for p in range(P) if p not in good.values()]
+    assert torch.equal(st[rest], pool[rest])
+    pkg.check_device_status(torch.device(DEV))  # the report was cleared
+
+
+def test_decode_strides_out_of_place_and_pool_slices(pkg):
+    B, Hqk, Hv, d = 6, 2, 4, 64
+    gen = torch.Generator().manual_seed(6)
+    qkv = torch.randn(B, Hqk * 2 + Hv, d, generator=gen).to(torch.bfloat16).to(DEV)
+    q, k, v = qkv[:, :Hqk], qkv[:, Hqk : 2 * Hqk], qkv[:, 2 * Hqk :]
+    g = (-torch.rand(Hv, B, generator=gen)).to(DEV).t()
+    layers = torch.randn(B, 3, Hv, d, d, generator=gen).to(DEV)
+    new = torch.full((B, Hv, d, d), float("nan"), device=DEV)
+    out = torch.zeros(B, 2, Hv, d, dtype=torch.bfloat16, device=DEV)
+    before = layers.clone()
+    pkg.lin_decode(q, k, v, g, layers[:, 1], out=out[:, 1], state_out=new, check=True)
+    assert torch.equal(layers, before) and bool((out[:, 0] == 0).all())
+    check_decode(out[:, 1].cpu(), new.cpu(), q.cpu(), k.cpu(), v.cpu(), g.cpu(), before[:, 1].cpu(), 1.0,
+                 torch.bfloat16)
+
+
+def test_decode_large_pool_offsets(pkg):
+    """Pages whose element offsets pass 32 bits."""
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB of device memory")
+    Hv, dk, dv = 32, 128, 128
+    pool = torch.empty((1 << 32) // (Hv * dk * dv) + 3, Hv, dk, dv, device=DEV)
+    P = pool.shape[0]
+    pages = [P - 1, 0, P - 2]
+    q, k, v, g = make((3,), 32, 32, dk, dv, torch.bfloat16, 7)
+    S = torch.randn(3, Hv, dk, dv, generator=torch.Generator().manual_seed(8))
+    pool[pages] = S.to(DEV)
+    o = pkg.lin_decode(*(x.to(DEV) for x in (q, k, v, g)), pool,
+                       index=torch.tensor(pages, dtype=torch.int32, device=DEV), check=True).cpu()
+    check_decode(o, pool[pages].cpu(), q, k, v, g, S, 1.0, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ prefill
+
+
+@pytest.mark.parametrize("T", [1, 2, 63, 64, 65, 127, 128, 129, 300])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128)])
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+def test_prefill(pkg, T, dk, dv, io):
+    B, Hqk, Hv = 2, 1, 2
+    q, k, v, g = make((B, T), Hqk, Hv, dk, dv, io, T + dk)
+    S0 = torch.randn(B, Hv, dk, dv, generator=torch.Generator().manual_seed(T)) if T % 2 else None
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV) if S0 is not None else None,
+                           scale=dk ** -0.5, check=True)
+    for b in range(B):
+        ref = steps(q[b], k[b], v[b], g[b], S0[b] if S0 is not None else torch.zeros(Hv, dk, dv), dk ** -0.5)
+        check_prefill(o[b].cpu(), S[b].cpu(), ref, io, k[b], v[b])
+
+
+@pytest.mark.parametrize("dv", [192, 256])
+@pytest.mark.parametrize("B,Hqk,Hv", [(1, 1, 1), (1, 1, 5), (3, 2, 4)])
+def test_prefill_wide_values_and_heads(pkg, dv, B, Hqk, Hv):
+    T, dk, io = 150, 128, torch.bfloat16
+    q, k, v, g = make((B, T), Hqk, Hv, dk, dv, io, dv)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), check=True)
+    for b in range(B):
+        ref = steps(q[b], k[b], v[b], g[b], torch.zeros(Hv, dk, dv), 1.0)
+        check_prefill(o[b].cpu(), S[b].cpu(), ref, io, k[b], v[b])
+
+
+@pytest.mark.parametrize("gate", ["token", "head"])
+@pytest.mark.parametrize("g_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gmin", [0.0, -0.01, -5.0])
+def test_prefill_gates(pkg, gate, g_dtype, gmin):
+    T, d, io = 200, 64, torch.bfloat16
+    q, k, v, g = make((1, T), 2, 2, d, d, io, 9, gmin=gmin, g_dtype=g_dtype, gate=gate)
+    S0 = torch.randn(1, 2, d, d)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), check=True)
+    gg = g[0] if gate == "token" else g.expand(T, 2)
+    check_prefill(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], gg, S0[0], 1.0), io, k[0], v[0])
+
+
+@pytest.mark.parametrize("g_reset", [float("-inf"), -200.0, -1e30])
+def test_prefill_resets(pkg, g_reset):
+    """A decay of zero at some tokens starts the sequence anew there, also inside a chunk."""
+    T, d, io = 260, 64, torch.bfloat16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 10)
+    g[0, [0, 5, 6, 127, 128, 200], 0] = g_reset
+    g[0, :, 1] = g_reset
+    S0 = torch.randn(1, 2, d, d)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), check=True)
+    check_prefill(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], S0[0], 1.0), io, k[0], v[0])
+
+
+def test_prefill_packed_ragged_with_pages(pkg):
+    Hqk, Hv, dk, dv, io = 1, 2, 128, 64, torch.float16
+    lens = [5, 0, 130, 1, 128, 257, 0, 64]
+    lead, tail = 3, 9  # rows before the first and behind the last sequence
+    T = lead + sum(lens) + tail
+    q, k, v, g = make((1, T), Hqk, Hv, dk, dv, io, 11)
+    # nothing of the rows outside may reach a sequence
+    for x in (q, k, v):
+        x[0, :lead] = float("nan")
+        x[0, T - tail :] = float("inf")
+    cu = [lead]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    P = 11
+    pool = torch.randn(P, Hv, dk, dv, generator=torch.Generator().manual_seed(12))
+    index = torch.tensor([4, 9, 0, -1, 10, 2, -3, 7], dtype=torch.int32)
+    st = pool.to(DEV)
+    out = torch.full((1, T, Hv, dv), 7.0, dtype=io, device=DEV)
+    o, fin = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st, scale=0.1, out=out, index=index.to(DEV),
+                             cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV), check=True)
+    assert fin is st and o is out
+    o, fin = o.cpu(), fin.cpu()
+    assert bool((o[0, :lead] == 7).all()) and bool((o[0, T - tail :] == 7).all())
+    kept = set(range(P))
+    for n, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        p = int(index[n])
+        S0 = pool[p] if p >= 0 else torch.zeros(Hv, dk, dv)
+        ref = steps(q[0, a:b], k[0, a:b], v[0, a:b], g[0, a:b], S0, 0.1)
+        if p >= 0:
+            kept.discard(p)
+            if b == a:
+                assert torch.equal(fin[p], pool[p])
+                continue
+        elif b == a:
+            continue
+        check_prefill(o[0, a:b], fin[p] if p >= 0 else ref[1], ref, io, k[0, a:b], v[0, a:b])
+    kept = sorted(kept)
+    assert torch.equal(fin[kept], pool[kept])
+
+
+def test_prefill_neighbours_of_other_sequences_stay_out(pkg):
+    """A sequence that ends inside a chunk, next to one of NaN and infinities."""
+    Hv, d, io = 1, 64, torch.bfloat16
+    lens = [37, 100, 91]
+    T = sum(lens)
+    q, k, v, g = make((1, T), Hv, Hv, d, d, io, 13)
+    for x in (q, k, v):
+        x[0, 37:87] = float("nan")
+        x[0, 87:137] = float("inf")
+    cu = torch.tensor([0, 37, 137, 228], dtype=torch.int32, device=DEV)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), cu_seqlens=cu, check=True)
+    for n, (a, b) in enumerate([(0, 37), (137, 228)]):
+        ref = steps(q[0, a:b], k[0, a:b], v[0, a:b], g[0, a:b], torch.zeros(Hv, d, d), 1.0)
+        check_prefill(o[0, a:b].cpu(), S[2 * n].cpu(), ref, io, k[0, a:b], v[0, a:b])
+
+
+def test_prefill_reports_bad_offsets_and_pages(pkg):
+    Hv, d, io, T = 1, 64, torch.bfloat16, 40
+    q, k, v, g = (x.to(DEV) for x in make((1, T), Hv, Hv, d, d, io, 14))
+    for cu in ([0, 41], [-1, 10], [0, 20, 10]):
+        fin = torch.full((len(cu) - 1, Hv, d, d), 3.0, device=DEV)
+        with pytest.raises(pkg.GDNError, match="index"):
+            pkg.lin_prefill(q, k, v, g, final_state=fin, check=True,
+                            cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+        assert bool((fin[-1] == 3).all())  # the unsound sequence, here the last, leaves no state
+    cu = torch.tensor([0, 10, 30, 40], dtype=torch.int32, device=DEV)
+    pool = torch.full((3, Hv, d, d), 3.0, device=DEV)
+    with pytest.raises(pkg.GDNError, match="index"):
+        pkg.lin_prefill(q, k, v, g, final_state=pool, cu_seqlens=cu, check=True,
+                        index=torch.tensor([1, 3, 1], dtype=torch.int32, device=DEV))
+    ref = steps(*(x[0, :10].cpu() for x in (q, k, v, g)), torch.zeros(Hv, d, d), 1.0)
+    assert float((pool[1].cpu().double() - ref[1]).abs().max()) < 1e-3
+    assert bool((pool[[0, 2]] == 3).all())
+
+
+def test_prefill_strided_views(pkg):
+    B, T, Hqk, Hv, d, io = 2, 70, 1, 2, 64, torch.bfloat16
+    gen = torch.Generator().manual_seed(15)
+    x = torch.randn(B, T, 2 * Hqk + Hv, d, generator=gen).to(io).to(DEV)
+    q, k, v = x[:, :, :Hqk], x[:, :, Hqk : 2 * Hqk], x[:, :, 2 * Hqk :]
+    g = (-torch.rand(Hv, T, B, generator=gen) * 0.1).to(DEV).permute(2, 1, 0)
+    layers = torch.randn(B, 2, Hv, d, d, generator=gen).to(DEV)
+    out = torch.zeros(B, T, 2, Hv, d, dtype=io, device=DEV)
+    S0 = layers[:, 1].clone()
+    o, fin = pkg.lin_prefill(q, k, v, g, layers[:, 1], out=out[:, :, 1], final_state=layers[:, 1], check=True)
+    assert bool((out[:, :, 0] == 0).all())
+    for b in range(B):
+        ref = steps(q[b].cpu(), k[b].cpu(), v[b].cpu(), g[b].cpu(), S0[b].cpu(), 1.0)
+        check_prefill(o[b].cpu(), fin[b].cpu(), ref, io, k[b].cpu(), v[b].cpu())
+
+
+def test_prefill_small_f16_values_keep_the_state(pkg):
+    """Values near f16's smallest normal numbers, decayed further within the chunk."""
+    T, d, io = 128, 64, torch.float16
+    q, k, v, g = make((1, T), 1, 1, d, d, io, 16, gmin=-0.1)
+    v = (v.float() * 2.0 ** -12).to(io)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), check=True)
+    check_prefill(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], torch.zeros(1, d, d), 1.0), io, k[0], v[0])
+
+
+def test_prefill_long_few_heads_equals_pieces(pkg):
+    """A long time axis over few heads against the same tokens in two calls, and sampled rows against 64 bits."""
+    T, d, io = 9000, 128, torch.bfloat16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 17, gmin=-0.02)
+    x = [t.to(DEV) for t in (q, k, v, g)]
+    o, S = pkg.lin_prefill(*x, scale=d ** -0.5, check=True)
+    cut = 4100
+    o1, S1 = pkg.lin_prefill(*(t[:, :cut] for t in x), scale=d ** -0.5, check=True)
+    o2, S2 = pkg.lin_prefill(*(t[:, cut:] for t in x), S1, scale=d ** -0.5, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), d ** -0.5)
+    check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0, -2000:], v[0])
+    check_prefill(torch.cat([o1, o2], 1)[0].cpu(), S2[0].cpu(), ref, io, k[0, -2000:], v[0])
+
+
+def test_graph_capture_on_another_stream(pkg):
+    """Prefill and decode captured together, replayed on new inputs."""
+    B, T, H, d, io = 2, 200, 2, 128, torch.bfloat16
+    sets = [[x.to(DEV) for x in make((B, T), H, H, d, d, io, s)] for s in (20, 21)]
+    tok = [[x.to(DEV) for x in make((B,), H, H, d, d, io, s)] for s in (22, 23)]
+    x, y = [t.clone() for t in sets[0]], [t.clone() for t in tok[0]]
+    st = torch.empty(B, H, d, d, device=DEV)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        pkg.lin_prefill(*x, final_state=st)
+        pkg.lin_decode(*y, st)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        o, _ = pkg.lin_prefill(*x, final_state=st)
+        od = pkg.lin_decode(*y, st)
+    for i in (1, 0):
+        for a, b in zip(x + y, sets[i] + tok[i]):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, S = pkg.lin_prefill(*sets[i])
+        want_d = pkg.lin_decode(*tok[i], S)
+        assert torch.equal(o, want) and torch.equal(od, want_d) and torch.equal(st, S)
+    pkg.check_device_status(torch.device(DEV))
