@@ -16,16 +16,20 @@
 //
 // Warps (19): R 0-3 (a row of the chunk per thread), V 4-7, S 8-15, TMA 16,
 // gates 17, MMA 18.  Per chunk, in the MMA warp's order:
-//   SC  scores = Q K^T             both from shared memory; R turns them into
+//   SC  scores = Q' K^T            Q' = scale e^G Q in TMEM (R); R turns them into
 //                                  P, packed over the scores' own columns
-//   LO  dS^T  = V''lo^T K          A from TMEM
-//   QS  O     = Q' S               Q' = scale e^G Q in TMEM (R), S^T in shared memory
-//   HI  dS^T += V''hi^T K          then S reads dS and rewrites S^T
-//   PV  O    += P V                then V packs O into the Q tile and stores it
-// V'' = e^(G_C - G_j) v is split into two parts of the I/O type, v'' = hi + lo,
-// because the state is kept to fp32 accuracy: one 8-bit part would leave 2^-9
-// of every term.  V writes both parts in turn to the same 64 columns, while the
-// tensor cores are at SC and QS.
+//   D0  dS^T  = V''^T K            of the chunk's first 64 tokens, V'' in TMEM (V)
+//   QS  O     = Q' S               S^T in shared memory
+//   D1  dS^T += V''^T K            of the others; then S reads dS and rewrites S^T
+//   PV  O    += P V                then S writes O out
+// All five take A from TMEM: a product with both operands in shared memory
+// reads it at its full rate, and other warps' reads then take five times as
+// long (4 ldmatrix.x4: 726 cycles against 141).
+// V'' = w v, w = e^(G_C - G_j), is split into two parts of the I/O type, hi +
+// lo, because the state is kept to fp32 accuracy: one part would leave half a
+// step of the I/O type of every term.  So is w, which makes both parts a few
+// packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo = (v w_hi -
+// hi) + v w_lo, the difference being exact.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -39,11 +43,15 @@ namespace {
 
 constexpr int kC = 128;             // tokens of a chunk
 constexpr int kTile = kC * 128;     // bytes of a [128][64] 16-bit tile
-constexpr int kThreads = 19 * 32;
-constexpr int kWarpV = 4, kWarpS = 8, kWarpTma = 16, kWarpGate = 17, kWarpMma = 18;
+constexpr int kThreads = 20 * 32;
+constexpr int kWarpV = 4, kWarpS = 8, kWarpTma = 16, kWarpGate = 17, kWarpMma = 18, kWarpStore = 19;
 constexpr float kLog2e = 1.4426950408889634f;
+// a wait sleeps for up to this long at a time, and ends after so many cycles
+constexpr uint32_t kSleepNs = 20000, kWaitCycles = 2000u * 1000u * 1000u;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
+// within this range e^(G_i - G_j) is taken as the product of e^G_i and e^-G_j
+constexpr float kNear = 100.f;
 
 // TMEM columns
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
@@ -61,24 +69,26 @@ struct Layout {
   static constexpr int kStages = 2;
   static constexpr int kS = kStages * kStage;              // S^T bf16 [BV][DK], 64-wide blocks
   static constexpr int kSBlock = BV * 128;
-  // O is staged in the chunk's Q tile where it fits
-  static constexpr bool kOInQ = BV <= DK;
-  static constexpr int kO = kS + DK / 64 * kSBlock;
-  static constexpr int kGate = kO + (kOInQ ? 0 : BV / 64 * kTile);
-  static constexpr int kGateStage = 2 * kC * 4;            // G, w
+  // O of a chunk is staged in its K tile (read last by D1), or in its V tile (read
+  // last by PV, and wanted again a little sooner) where the K tile is too small
+  static constexpr bool kOInK = DK >= BV;
+  static constexpr int kO = kOInK ? kK : kV;
+  static constexpr int kGate = kS + DK / 64 * kSBlock;
+  static constexpr int kGateStage = 2 * kC * 4;            // G or e^-G, w
   static constexpr int kBars = kGate + 2 * kGateStage;
   static constexpr int kBytes = kBars + 256;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
 struct Bars {
-  uint64_t full[2], empty_kv[2], empty_q[2];
+  uint64_t full[2], empty_k[2], empty_v[2], empty_q[2];
   uint64_t gfull[2], gempty[2];
-  uint64_t sc_done, q_ready, p_ready, pv_done;
-  uint64_t v_ready, v_free, o_free, ds_done, s_ready, drain;
+  uint64_t sc_done, q_ready, qs_done, p_ready, pv_done;
+  uint64_t v_ready, v_free, ds_done, s_ready;
+  uint64_t o_free, o_staged, zeroed, drain;
   float gamma[2];
+  int near_one[2];  // the chunk's e^G and e^-G both stay well inside fp32
   uint32_t tmem;
-  uint32_t pad;
 };
 static_assert(sizeof(Bars) <= 256, "barriers");
 
@@ -117,6 +127,18 @@ __device__ Seq find_seq(const lin_prefill_args_t& a, int n, bool reporter) {
   return s;
 }
 
+// Shared-memory loads that stay where they are written: ahead of the arithmetic.
+template <typename T>
+__device__ __forceinline__ void lds128(const void* p, T* x) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(x);
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3])
+               : "r"(smem_u32(p)));
+}
+__device__ __forceinline__ void lds64(const void* p, uint32_t* u) {
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(u[0]), "=r"(u[1]) : "r"(smem_u32(p)));
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -129,18 +151,27 @@ __device__ __forceinline__ float log2_gate(float g) {
   return x < kLowest ? kLowest : x;
 }
 
-// Waits for a phase; on a timeout reports `bits` and returns false.  For one
-// thread; wait() is for a whole warp, whose lanes all get the same answer.
-__device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t bits) {
-  if (mbar_wait_bounded(bar, parity)) return true;
-  report(status, bits);
-  return false;
+// Waits for a phase, asleep in the barrier unit for most of it; false after about
+// a second.  Short on purpose: two dozen copies of it share the instruction cache
+// with the roles' loops.  wait1() is for one thread; wait() for a whole warp,
+// whose lanes all get the same answer.
+__device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_u32(bar);
+  const uint32_t t0 = static_cast<uint32_t>(clock());
+  uint32_t ok;
+  do {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(at), "r"(parity), "r"(kSleepNs)
+        : "memory");
+  } while (!ok && static_cast<uint32_t>(clock()) - t0 < kWaitCycles);
+  return ok != 0;
 }
-__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, uint32_t* status, uint32_t bits) {
-  const bool ok = mbar_wait_bounded(bar, parity);
-  if (__all_sync(0xffffffffu, ok)) return true;
-  report(status, bits);
-  return false;
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait1(bar, parity));
 }
 
 template <int DK, int BV, typename IO>
@@ -162,20 +193,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar.full[s], 1);
-      mbar_init(&bar.empty_kv[s], 1);
-      mbar_init(&bar.empty_q[s], 1);
+      mbar_init(&bar.empty_k[s], 1);
+      mbar_init(&bar.empty_v[s], 1);
+      mbar_init(&bar.empty_q[s], 4);
       mbar_init(&bar.gfull[s], 1);
       mbar_init(&bar.gempty[s], 16);
     }
     mbar_init(&bar.sc_done, 1);
     mbar_init(&bar.q_ready, 4);
+    mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
     mbar_init(&bar.pv_done, 1);
     mbar_init(&bar.v_ready, 4);
     mbar_init(&bar.v_free, 1);
-    mbar_init(&bar.o_free, 4);
     mbar_init(&bar.ds_done, 1);
     mbar_init(&bar.s_ready, 8);
+    mbar_init(&bar.o_free, 4);
+    mbar_init(&bar.o_staged, 4);
+    mbar_init(&bar.zeroed, 4);
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
   }
@@ -189,6 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = bar.tmem;
   const uint32_t sb = smem_u32(smem);
   uint32_t* const status = a.status;
+  bool ok = true;
 
   if (warp < kWarpV) {
     // ------------------------------------------------ R: a row per thread
@@ -199,60 +235,85 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t ph = (c >> 1) & 1;
       const unsigned char* stage = smem + st * L::kStage;
       const float* G = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage);
-      if (!wait(&bar.gfull[st], ph, status, GDN_DEVERR_FULL_TIMEOUT)) break;
-      if (!wait(&bar.full[st], ph, status, GDN_DEVERR_FULL_TIMEOUT)) break;
-      // Q' = scale e^G Q over the columns that the last chunk's QS has read
-      if (c && !wait(&bar.pv_done, (c - 1) & 1, status, GDN_DEVERR_MMA_TIMEOUT)) break;
+      if (!(ok = wait(&bar.gfull[st], ph))) break;
+      if (!(ok = wait(&bar.full[st], ph))) break;
+      // the columns that the last chunk's QS has read
+      if (c && !(ok = wait(&bar.qs_done, (c - 1) & 1))) break;
       tc::fence_after_sync();
-      const float Gi = G[row];
-      const float f = a.scale * ex2(Gi);
+      const bool near_one = bar.near_one[st];
+      const float Gi = G[row];  // e^-G when near one
+      const float f = a.scale * (near_one ? __frcp_rn(Gi) : ex2(Gi));
+      const uint32_t f_hi = tc::pack2<true>(f, f);
+      const uint32_t f_lo = tc::pack2<true>(f - tc::unpack_lo<true>(f_hi), f - tc::unpack_lo<true>(f_hi));
+      const auto put_q = [&](bool scaled) {
+#pragma unroll 1
+        for (int b = 0; b < DK / 64; ++b) {
+          uint32_t u[2][16];
 #pragma unroll
-      for (int b = 0; b < DK / 32; ++b) {
-        uint32_t u[16];
+          for (int e = 0; e < 8; ++e)
+            lds128(stage + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
+          if (scaled) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int chunk = (b & 1) * 4 + e;
-          const uint4 x = *reinterpret_cast<const uint4*>(stage + L::kQ + (b >> 1) * kTile + tc::sw128_offset(row, chunk));
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            u[e * 4 + i] = tc::pack2<true>(f * tc::unpack_lo<BF16>(w[i]), f * tc::unpack_hi<BF16>(w[i]));
+            for (int i = 0; i < 32; ++i) {
+              uint32_t& w = u[i >> 4][i & 15];
+              w = BF16 ? tc::fma2<true>(w, f_hi, tc::mul2<true>(w, f_lo))
+                       : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
+            }
+          }
+          tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
+          tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
         }
-        tc::tmem_st16(tmem + lanes + kTmQ + b * 16, u);
-      }
-      tc::tmem_wait_st();
+        tc::tmem_wait_st();
+      };
+      // bf16 near one: SC and QS both take Q'.  Else SC takes Q as it is, since
+      // e^G could leave the type's range, and Q' follows it.
+      const bool shared_q = BF16 && near_one;
+      put_q(shared_q);
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.q_ready);
 
-      if (!wait(&bar.sc_done, c & 1, status, GDN_DEVERR_MMA_TIMEOUT)) break;
+      if (!(ok = wait(&bar.sc_done, c & 1))) break;
       tc::fence_after_sync();
-      // P in the I/O type over the scores: columns [16 b, 16 b + 16) go to [8 b, 8 b + 8)
+      if (!shared_q) put_q(true);
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&bar.q_ready);
+        mbar_arrive(&bar.empty_q[st]);
+      }
+      // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
+#pragma unroll 1
+      for (int b = 0; b < 4; ++b) {
+        uint32_t u[16];
+        if (b <= warp) {
+          // the loads first: shared memory answers late while the products read it
+          float x[2][16], d[32];
+          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32, x[0]);
+          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        uint32_t u[8];
-        if (b * 16 < warp * 32 + 32) {
-          float s[16];
-          tc::tmem_ld16(tmem + lanes + kTmSC + b * 16, s);
-          float d[16];
+          for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
+          if (!near_one) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4 g = *reinterpret_cast<const float4*>(G + b * 16 + e * 4);
-            d[e * 4 + 0] = a.scale * ex2(Gi - g.x);
-            d[e * 4 + 1] = a.scale * ex2(Gi - g.y);
-            d[e * 4 + 2] = a.scale * ex2(Gi - g.z);
-            d[e * 4 + 3] = a.scale * ex2(Gi - g.w);
+            for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
+          } else if (!BF16) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) d[e] *= f;
           }
           tc::tmem_wait_ld();
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = b * 16 + e <= row ? s[e] * d[e] : 0.f;
+          for (int e = 0; e < 32; ++e) d[e] *= x[e >> 4][e & 15];
+          if (b == warp) {  // on the diagonal
 #pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = tc::pack2<BF16>(s[2 * e], s[2 * e + 1]);
+            for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = tc::pack2<BF16>(d[2 * e], d[2 * e + 1]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) u[e] = 0;
+          for (int e = 0; e < 16; ++e) u[e] = 0;
         }
-        tc::tmem_st8(tmem + lanes + kTmSC + b * 8, u);
+        tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
@@ -263,46 +324,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < kWarpS) {
-    // ------------------------------------------------ V: V'' parts, and the output rows
-    const int vt = tid - kWarpV * 32, quarter = warp - kWarpV;
+    // ------------------------------------------------ V: V'' parts
+    const int quarter = warp - kWarpV, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const bool has_rows = quarter * 32 < BV;
-    // A warp whose wait ran out keeps to the group's barriers until output(),
-    // where the group agrees to stop.
-    bool ok = true, stop = false;
-    // part 0: lo, part 1: hi
-    const auto parts = [&](int c, int part) {
+    // tokens [64 half, 64 half + 64) of chunk c: both parts
+    const auto parts = [&](int c, int half) {
       const int st = c & 1;
       const uint32_t tile = sb + st * L::kStage + L::kV;
-      const float* w = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage) + kC;
+      const uint2* w = reinterpret_cast<const uint2*>(smem + L::kGate + st * L::kGateStage + kC * 4) + half * 32 + (lane & 3);
       if (has_rows) {
+        uint32_t ww[4][4];  // (hi, lo) of tokens 2 l, 2 l + 1 and 2 l + 8, 2 l + 9 of each 16, l = lane % 4
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int dv = quarter * 32 + half * 16;  // of this warp's 16 rows
+        for (int tb = 0; tb < 4; ++tb) {
+          lds64(w + tb * 8, ww[tb]);
+          lds64(w + tb * 8 + 4, ww[tb] + 2);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int dv = quarter * 32 + i * 16;  // of this warp's 16 rows
           const uint32_t block = tile + (dv >> 6) * kTile;
           const int chunk = ((dv & 63) >> 3) + ((lane >> 3) & 1);
+          uint32_t r[4][4], hi[16], lo[16];
 #pragma unroll
-          for (int t0 = 0; t0 < kC; t0 += 64) {
-            uint32_t u[16];
+          for (int tb = 0; tb < 4; ++tb)
+            tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[tb]);
 #pragma unroll
-            for (int tb = 0; tb < 4; ++tb) {
-              const int t = t0 + tb * 16;
-              uint32_t r[4];
-              tc::ldsm_x4_trans(block + tc::sw128_offset(t + (lane >> 4) * 8 + (lane & 7), chunk), r);
-              const float2 w0 = *reinterpret_cast<const float2*>(w + t + 2 * (lane & 3));
-              const float2 w1 = *reinterpret_cast<const float2*>(w + t + 8 + 2 * (lane & 3));
-#pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                const float2 ww = m < 2 ? w0 : w1;
-                const float x = ww.x * tc::unpack_lo<BF16>(r[m]), y = ww.y * tc::unpack_hi<BF16>(r[m]);
-                uint32_t z = tc::pack2<BF16>(x, y);
-                if (part == 0)  // what the leading part leaves, exact in fp32
-                  z = tc::pack2<BF16>(x - tc::unpack_lo<BF16>(z), y - tc::unpack_hi<BF16>(z));
-                u[tb * 4 + m] = z;
-              }
-            }
-            tc::tmem_st_16x128b_x8(tmem + lanes + (static_cast<uint32_t>(half * 16) << 16) + kTmV + t0 / 2, u);
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t v = r[e >> 2][e & 3], w_hi = ww[e >> 2][e & 2], w_lo = ww[e >> 2][(e & 2) + 1];
+            hi[e] = tc::fma2<BF16>(v, w_hi, tc::mul2<BF16>(v, w_lo));
+            lo[e] = tc::fma2<BF16>(v, w_lo, tc::fma2<BF16>(v, w_hi, hi[e] ^ 0x80008000u));
           }
+          const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + kTmV;
+          tc::tmem_st_16x128b_x8(to, lo);
+          tc::tmem_st_16x128b_x8(to + 32, hi);
         }
         tc::tmem_wait_st();
       }
@@ -310,86 +365,79 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.v_ready);
     };
-    // O of chunk c: packed into shared memory, then out
+    // O of chunk c: a token per thread, packed into shared memory
     const auto output = [&](int c) {
       const int st = c & 1;
-      unsigned char* o = smem + (L::kOInQ ? st * L::kStage + L::kQ : L::kO);
-      ok = ok && wait(&bar.pv_done, c & 1, status, GDN_DEVERR_MMA_TIMEOUT);
-      stop = named_barrier_or(1, 128, !ok);
-      if (stop) return;
+      unsigned char* o = smem + st * L::kStage + L::kO;
+      if (!wait(&bar.pv_done, c & 1)) return false;
       tc::fence_after_sync();
-      if (!L::kOInQ && c) {  // the last store has read the tile
-        if (vt == 0) bulk_wait_read();
-        tc::group_sync(1, 128);
-      }
-#pragma unroll
-      for (int b = 0; b < BV / 16; ++b) {
-        float x[16];
-        tc::tmem_ld16(tmem + lanes + kTmO + b * 16, x);
+#pragma unroll 1
+      for (int b = 0; b < BV / 32; ++b) {
+        float x[2][16];
+        tc::tmem_ld16(tmem + lanes + kTmO + b * 32, x[0]);
+        tc::tmem_ld16(tmem + lanes + kTmO + b * 32 + 16, x[1]);
         tc::tmem_wait_ld();
-        const uint32_t at = smem_u32(o) + (b >> 2) * kTile;
+        const uint32_t to = smem_u32(o) + (b >> 1) * kTile;
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          tc::sts128(at + tc::sw128_offset(vt, (b & 3) * 2 + e), tc::pack2<BF16>(x[8 * e], x[8 * e + 1]),
-                     tc::pack2<BF16>(x[8 * e + 2], x[8 * e + 3]), tc::pack2<BF16>(x[8 * e + 4], x[8 * e + 5]),
-                     tc::pack2<BF16>(x[8 * e + 6], x[8 * e + 7]));
+        for (int e = 0; e < 4; ++e) {
+          const float* y = &x[e >> 1][(e & 1) * 8];
+          tc::sts128(to + tc::sw128_offset(row, (b & 1) * 4 + e), tc::pack2<BF16>(y[0], y[1]), tc::pack2<BF16>(y[2], y[3]),
+                     tc::pack2<BF16>(y[4], y[5]), tc::pack2<BF16>(y[6], y[7]));
+        }
       }
       tc::fence_before_sync();
       tc::fence_proxy_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.o_free);
-      tc::group_sync(1, 128);
-      const int rows = min(kC, seq.len - c * kC);
-      if (rows == kC) {
-        if (vt == 0) {
-          for (int b = 0; b < BV / 64; ++b)
-            tc::tma_store_4d(&map_o, o + b * kTile, vb * BV + b * 64, h, seq.start + c * kC, batch);
-          bulk_commit();
-          if (L::kOInQ) {
-            bulk_wait_read();
-            mbar_arrive(&bar.empty_q[st]);
-          }
-        }
-      } else {  // the rows behind belong to another sequence, or to nobody
+      if (lane == 0) {
+        mbar_arrive(&bar.o_staged);
+        mbar_arrive(&bar.o_free);
+      }
+      const int rows = seq.len - c * kC;
+      if (rows < kC) {  // the rows behind belong to another sequence, or to nobody
+        if (!wait(&bar.o_staged, c & 1)) return false;
         IO* dst = static_cast<IO*>(a.o) + batch * a.o_sb + static_cast<int64_t>(seq.start + c * kC) * a.o_st + h * a.o_sh +
                   vb * BV;
         constexpr int kPer = BV / 8;  // 16-byte pieces of a row
-        for (int i = vt; i < rows * kPer; i += 128) {
+        for (int i = row; i < rows * kPer; i += 128) {
           const int r = i / kPer, piece = i - r * kPer;
           const uint4 x = *reinterpret_cast<const uint4*>(o + (piece >> 3) * kTile + tc::sw128_offset(r, piece & 7));
           *reinterpret_cast<uint4*>(dst + r * a.o_st + piece * 8) = x;
         }
       }
-      if (!L::kOInQ && vt == 0) mbar_arrive(&bar.empty_q[st]);
+      return true;
     };
-    for (int c = 0; c < chunks && !stop; ++c) {
-      const int st = c & 1;
-      const uint32_t ph = (c >> 1) & 1;
-      ok = ok && wait(&bar.gfull[st], ph, status, GDN_DEVERR_FULL_TIMEOUT) &&
-           wait(&bar.full[st], ph, status, GDN_DEVERR_FULL_TIMEOUT);
-      const int rows = min(kC, seq.len - c * kC);
-      if (rows < kC) {
-        // rows of the next sequence, or outside: zero, whatever they hold, since
-        // 0 x NaN would reach the sums over the chunk's tokens
-        unsigned char* stage = smem + st * L::kStage;
-        if (ok)
+    // Two steps a chunk, 64 tokens each, the last chunk's output between them.
+    // One call site each keeps the kernel's code within the instruction cache.
+#pragma unroll 1
+    for (int step = 0; step <= 2 * chunks; ++step) {
+      const int c = step >> 1, half = step & 1, st = c & 1;
+      if (c < chunks) {
+      if (half == 0) {
+        const uint32_t ph = (c >> 1) & 1;
+        if (!(ok = wait(&bar.gfull[st], ph))) break;
+        if (!(ok = wait(&bar.full[st], ph))) break;
+        const int rows = seq.len - c * kC;
+        if (rows < kC) {
+          // rows of the next sequence, or outside: zero, whatever they hold, since
+          // 0 x NaN would reach the sums over the chunk's tokens
+          unsigned char* stage = smem + st * L::kStage;
           for (int r = rows + quarter; r < kC; r += 4)
             for (int i = lane; i < (DK + BV) / 8; i += 32)
-              *reinterpret_cast<uint4*>(stage + L::kK + (i >> 3) * kTile + tc::sw128_offset(r, i & 7)) = make_uint4(0, 0, 0, 0);
-        tc::fence_proxy_async();
-        tc::group_sync(1, 128);
+              *reinterpret_cast<uint4*>(stage + L::kK + (i >> 3) * kTile + tc::sw128_offset(r, i & 7)) =
+                  make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bar.zeroed);
+          if (!(ok = wait(&bar.zeroed, 0))) break;  // only the last chunk is short
+        }
       }
-      ok = ok && (c == 0 || wait(&bar.v_free, 1, status, GDN_DEVERR_MMA_TIMEOUT));
+      if (step && !(ok = wait(&bar.v_free, half ^ 1))) break;
       tc::fence_after_sync();
-      if (ok) parts(c, 0);
-      if (c) output(c - 1);
-      ok = ok && wait(&bar.v_free, 0, status, GDN_DEVERR_MMA_TIMEOUT);
-      tc::fence_after_sync();
-      if (ok) parts(c, 1);
-      if (lane == 0) mbar_arrive(&bar.gempty[st]);
+      parts(c, half);
+      if (half && lane == 0) mbar_arrive(&bar.gempty[st]);
+      }
+      if (c && !half && !(ok = output(c - 1))) break;
     }
-    if (chunks && !stop) output(chunks - 1);
-    if (vt == 0) bulk_wait_all();
   } else if (warp < kWarpTma) {
     // ------------------------------------------------ S: the state, a value column per thread
     const int quarter = warp & 3, half = (warp - kWarpS) >> 2;
@@ -403,8 +451,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float* from = a.initial_state + (load ? seq.page * a.initial_sp + at : 0);
 #pragma unroll
     for (int i = 0; i < kN; ++i) S[i] = load ? from[static_cast<int64_t>(i) * a.dv] : 0.f;
-    const auto publish = [&]() {  // S^T rounded to bf16, the QS product's operand
-      if (has_rows) {
+    // the state before chunk 0, then after each chunk
+#pragma unroll 1
+    for (int c = -1; c < chunks; ++c) {
+      if (c >= 0) {
+        const int st = c & 1;
+        ok = wait(&bar.gfull[st], (c >> 1) & 1) && wait(&bar.ds_done, c & 1);
+        if (!ok) break;
+        tc::fence_after_sync();
+        const float gamma = bar.gamma[st];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bar.gempty[st]);
+        if (has_rows) {
+#pragma unroll
+          for (int b = 0; b < kN / 16; ++b) {
+            float d[16];
+            tc::tmem_ld16(tmem + lanes + kTmDS + half * kN + b * 16, d);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], d[e]);
+          }
+        }
+      }
+      if (has_rows) {  // S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
@@ -417,29 +486,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.s_ready);
-    };
-    publish();
-    bool ok = true;
-    for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1;
-      ok = wait(&bar.gfull[st], (c >> 1) & 1, status, GDN_DEVERR_FULL_TIMEOUT) &&
-           wait(&bar.ds_done, c & 1, status, GDN_DEVERR_MMA_TIMEOUT);
-      if (!ok) break;
-      tc::fence_after_sync();
-      const float gamma = bar.gamma[st];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.gempty[st]);
-      if (has_rows) {
-#pragma unroll
-        for (int b = 0; b < kN / 16; ++b) {
-          float d[16];
-          tc::tmem_ld16(tmem + lanes + kTmDS + half * kN + b * 16, d);
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], d[e]);
-        }
-      }
-      publish();
     }
     if (ok && has_rows && seq.page >= 0 && seq.len >= 0) {
       float* to = a.final_state + seq.page * a.final_sp + at;
@@ -453,38 +499,52 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = c & 1;
         unsigned char* stage = smem + st * L::kStage;
         const int t = seq.start + c * kC;
-        if (c >= 2 && !wait1(&bar.empty_kv[st], ((c >> 1) & 1) ^ 1, status, GDN_DEVERR_EMPTY_TIMEOUT)) break;
+        const uint32_t ph = ((c >> 1) & 1) ^ 1;
+        // In the order in which the tiles come free.  The barrier is armed for the
+        // stage only once its Q tile is free, and so the chunk before complete.
+        if (c >= 2 && !(ok = wait1(&bar.empty_q[st], ph))) break;
         mbar_arrive_expect_tx(&bar.full[st], L::kStage);
-        for (int b = 0; b < DK / 64; ++b) tc::tma_load_4d(stage + L::kK + b * kTile, &map_k, b * 64, hq, t, batch, &bar.full[st]);
-        for (int b = 0; b < BV / 64; ++b)
-          tc::tma_load_4d(stage + L::kV + b * kTile, &map_v, vb * BV + b * 64, h, t, batch, &bar.full[st]);
-        if (c >= 2 && !wait1(&bar.empty_q[st], ((c >> 1) & 1) ^ 1, status, GDN_DEVERR_EMPTY_TIMEOUT)) {
-          // give the rest of the stage up, so that the drain below ends on what was issued
+        for (int b = 0; b < DK / 64; ++b) tc::tma_load_4d(stage + L::kQ + b * kTile, &map_q, b * 64, hq, t, batch, &bar.full[st]);
+        uint32_t missing = (DK + BV) / 64 * kTile;
+        if (c < 2 || wait1(&bar.empty_v[st], ph)) {
+          for (int b = 0; b < BV / 64; ++b)
+            tc::tma_load_4d(stage + L::kV + b * kTile, &map_v, vb * BV + b * 64, h, t, batch, &bar.full[st]);
+          missing -= BV / 64 * kTile;
+          if (c < 2 || wait1(&bar.empty_k[st], ph)) {
+            for (int b = 0; b < DK / 64; ++b)
+              tc::tma_load_4d(stage + L::kK + b * kTile, &map_k, b * 64, hq, t, batch, &bar.full[st]);
+            missing = 0;
+          }
+        }
+        if (missing) {  // given up: the drain below ends on what was issued
           asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&bar.full[st])),
-                       "r"(static_cast<uint32_t>(L::kK))
+                       "r"(missing)
                        : "memory");
+          ok = false;
           ++c;
           break;
         }
-        for (int b = 0; b < DK / 64; ++b) tc::tma_load_4d(stage + L::kQ + b * kTile, &map_q, b * 64, hq, t, batch, &bar.full[st]);
       }
       // no copy may be in flight when the shared memory is released
       for (int j = max(0, c - 2); j < c; ++j)
-        if (!wait1(&bar.full[j & 1], (j >> 1) & 1, status, GDN_DEVERR_DRAIN_TIMEOUT)) break;
+        if (!wait1(&bar.full[j & 1], (j >> 1) & 1)) {
+          ok = false;
+          break;
+        }
     }
   } else if (warp == kWarpGate) {
     // ------------------------------------------------ gates: 4 tokens per lane
     const int64_t g0 = batch * a.g_sb + h * a.g_sh;
-    const auto fetch = [&](int c, float (&x)[4]) {
+    float x[4], next[4];
+#pragma unroll 1
+    for (int c = -1; c < chunks; ++c) {  // a chunk's gates are fetched while the one before is at work
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int t = c * kC + lane * 4 + e;
-        x[e] = t < seq.len ? load_any(a.g, g0 + static_cast<int64_t>(seq.start + t) * a.g_st, a.g_dtype) : 0.f;
+        x[e] = next[e];
+        const int t = (c + 1) * kC + lane * 4 + e;
+        next[e] = t < seq.len ? load_any(a.g, g0 + static_cast<int64_t>(seq.start + t) * a.g_st, a.g_dtype) : 0.f;
       }
-    };
-    float x[4];
-    if (chunks) fetch(0, x);
-    for (int c = 0; c < chunks; ++c) {
+      if (c < 0) continue;
       const int st = c & 1;
       float* G = reinterpret_cast<float*>(smem + L::kGate + st * L::kGateStage);
       // cumulative in fp64: differences of far sums keep their small part
@@ -499,83 +559,117 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane >= off) inc += y;
       }
       const double before = inc - s[3], end = __shfl_sync(0xffffffffu, inc, 31);
-      if (c + 1 < chunks) fetch(c + 1, x);
-      if (c >= 2 && !wait(&bar.gempty[st], ((c >> 1) & 1) ^ 1, status, GDN_DEVERR_EMPTY_TIMEOUT)) break;
-      float4 gv, wv;
-      float* gp = &gv.x;
-      float* wp = &wv.x;
+      if (c >= 2 && !(ok = wait(&bar.gempty[st], ((c >> 1) & 1) ^ 1))) break;
+      float far = 0.f, gv[4], wv[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const double Gt = before + s[e];
-        gp[e] = static_cast<float>(Gt);
-        wp[e] = c * kC + lane * 4 + e < seq.len ? exp2f(static_cast<float>(end - Gt)) : 0.f;
+        gv[e] = static_cast<float>(Gt);
+        wv[e] = c * kC + lane * 4 + e < seq.len ? ex2(static_cast<float>(end - Gt)) : 0.f;
+        far = fmaxf(far, fabsf(gv[e]));
       }
-      *reinterpret_cast<float4*>(G + lane * 4) = gv;
-      *reinterpret_cast<float4*>(G + kC + lane * 4) = wv;
-      if (lane == 0) bar.gamma[st] = exp2f(static_cast<float>(end));
+      const bool near_one = __all_sync(0xffffffffu, far <= kNear);
+      if (near_one) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) gv[e] = ex2(-gv[e]);
+      }
+      *reinterpret_cast<float4*>(G + lane * 4) = make_float4(gv[0], gv[1], gv[2], gv[3]);
+      // the weights of two tokens in two parts of the I/O type: (hi, hi), (lo, lo)
+      uint32_t wp[4];
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        wp[e] = tc::pack2<BF16>(wv[e], wv[e + 1]);
+        wp[e + 1] = tc::pack2<BF16>(wv[e] - tc::unpack_lo<BF16>(wp[e]), wv[e + 1] - tc::unpack_hi<BF16>(wp[e]));
+      }
+      *reinterpret_cast<uint4*>(G + kC + lane * 4) = make_uint4(wp[0], wp[1], wp[2], wp[3]);
+      if (lane == 0) {
+        bar.gamma[st] = ex2(static_cast<float>(end));
+        bar.near_one[st] = near_one;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.gfull[st]);
     }
-  } else if (lane == 0) {
+  } else if (warp == kWarpStore) {
+    if (lane == 0) {  // whole chunks of O leave by TMA; V writes a short one
+      for (int c = 0; c < chunks && seq.len - c * kC >= kC; ++c) {
+        const int st = c & 1;
+        if (!(ok = wait1(&bar.o_staged, c & 1))) break;
+        for (int b = 0; b < BV / 64; ++b)
+          tc::tma_store_4d(&map_o, smem + st * L::kStage + L::kO + b * kTile, vb * BV + b * 64, h, seq.start + c * kC, batch);
+        bulk_commit();
+        bulk_wait_read();
+        mbar_arrive(L::kOInK ? &bar.empty_k[st] : &bar.empty_v[st]);
+      }
+      bulk_wait_all();
+    }
+  } else if (warp == kWarpMma && lane == 0) {
     // ------------------------------------------------ MMA
     constexpr uint32_t kIdSC = tc::idesc_f16(128, kC, false, false, BF16);
     constexpr uint32_t kIdDS = tc::idesc_f16(128, DK, false, true, BF16);
     constexpr uint32_t kIdQS = tc::idesc_f16(128, BV, false, false, true);
     constexpr uint32_t kIdPV = tc::idesc_f16(128, BV, false, true, BF16);
-    bool ok = true;
-    for (int c = 0; c < chunks; ++c) {
+        for (int c = 0; c < chunks; ++c) {
       const int st = c & 1;
-      const uint32_t q = sb + st * L::kStage + L::kQ, k = sb + st * L::kStage + L::kK, v = sb + st * L::kStage + L::kV;
-      const auto add_ds = [&](bool first) {
-#pragma unroll
-        for (int s = 0; s < kC / 16; ++s)
-          tc::mma_tmem_a(tmem + kTmDS, tmem + kTmV + s * 8, tc::mnmajor_desc(k, kTile, s), kIdDS, !first || s > 0);
+      // step s of an operand lies a constant number of 16-byte units after step 0
+      const uint32_t stage = sb + st * L::kStage;
+      const uint64_t k = tc::kmajor_desc(stage + L::kK, kTile, 0);
+      const uint64_t kt = tc::mnmajor_desc(stage + L::kK, kTile, 0), v = tc::mnmajor_desc(stage + L::kV, kTile, 0);
+      const uint64_t sT = tc::kmajor_desc(sb + L::kS, L::kSBlock, 0);
+      const auto along = [](int s, int block) { return static_cast<uint64_t>(((s >> 2) * block + (s & 3) * 32) >> 4); };
+      const auto add_ds = [&](int half) {  // 64 tokens: the small parts, then the large ones
+#pragma unroll 2
+        for (int s = 0; s < 8; ++s)
+          tc::mma_tmem_a(tmem + kTmDS, tmem + kTmV + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
       };
-      ok = wait1(&bar.full[st], (c >> 1) & 1, status, GDN_DEVERR_FULL_TIMEOUT) &&
-           (c == 0 || wait1(&bar.pv_done, (c - 1) & 1, status, GDN_DEVERR_MMA_TIMEOUT));
+      ok = wait1(&bar.full[st], (c >> 1) & 1) &&
+           wait1(&bar.q_ready, 0) &&
+           (c == 0 || wait1(&bar.pv_done, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 2
       for (int s = 0; s < DK / 16; ++s)
-        tc::mma(tmem + kTmSC, tc::kmajor_desc(q, kTile, s), tc::kmajor_desc(k, kTile, s), kIdSC, s > 0);
+        tc::mma_tmem_a(tmem + kTmSC, tmem + kTmQ + s * 8, k + along(s, kTile), kIdSC, s > 0);
       tc::commit(&bar.sc_done);
 
-      ok = wait1(&bar.s_ready, c & 1, status, GDN_DEVERR_MMA_TIMEOUT) &&
-           wait1(&bar.v_ready, 0, status, GDN_DEVERR_MMA_TIMEOUT);
+      ok = wait1(&bar.s_ready, c & 1) &&
+           wait1(&bar.v_ready, 0);
       if (!ok) break;
       tc::fence_after_sync();
-      add_ds(true);
+      add_ds(0);
       tc::commit(&bar.v_free);
 
-      ok = wait1(&bar.q_ready, c & 1, status, GDN_DEVERR_MMA_TIMEOUT) &&
-           (c == 0 || wait1(&bar.o_free, (c - 1) & 1, status, GDN_DEVERR_MMA_TIMEOUT));
+      ok = wait1(&bar.q_ready, 1) &&
+           (c == 0 || wait1(&bar.o_free, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 2
       for (int s = 0; s < DK / 16; ++s)
-        tc::mma_tmem_a(tmem + kTmO, tmem + kTmQ + s * 8, tc::kmajor_desc(sb + L::kS, L::kSBlock, s), kIdQS, s > 0);
+        tc::mma_tmem_a(tmem + kTmO, tmem + kTmQ + s * 8, sT + along(s, L::kSBlock), kIdQS, s > 0);
+      tc::commit(&bar.qs_done);
 
-      ok = wait1(&bar.v_ready, 1, status, GDN_DEVERR_MMA_TIMEOUT);
+      ok = wait1(&bar.v_ready, 1);
       if (!ok) break;
       tc::fence_after_sync();
-      add_ds(false);
+      add_ds(1);
       tc::commit(&bar.v_free);
       tc::commit(&bar.ds_done);
 
-      ok = wait1(&bar.p_ready, c & 1, status, GDN_DEVERR_MMA_TIMEOUT);
+      ok = wait1(&bar.p_ready, c & 1);
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll
+#pragma unroll 2
       for (int s = 0; s < kC / 16; ++s)
-        tc::mma_tmem_a(tmem + kTmO, tmem + kTmSC + s * 8, tc::mnmajor_desc(v, kTile, s), kIdPV, true);
+        tc::mma_tmem_a(tmem + kTmO, tmem + kTmSC + s * 8, v + s * 128, kIdPV, true);
       tc::commit(&bar.pv_done);
-      tc::commit(&bar.empty_kv[st]);
+      tc::commit(L::kOInK ? &bar.empty_v[st] : &bar.empty_k[st]);
     }
     if (!ok) {  // products in flight end before the tensor memory is released
       tc::commit(&bar.drain);
-      wait1(&bar.drain, 0, status, GDN_DEVERR_DRAIN_TIMEOUT);
+      wait1(&bar.drain, 0);
     }
   }
+  // a wait ran out: for a free slot, or for what the other warps do
+  if (!ok) report(status, warp == kWarpTma || warp == kWarpGate ? GDN_DEVERR_EMPTY_TIMEOUT : GDN_DEVERR_MMA_TIMEOUT);
   __syncwarp();
   tc::fence_before_sync();
   __syncthreads();
