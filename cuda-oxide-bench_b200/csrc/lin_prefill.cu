@@ -46,14 +46,13 @@ constexpr int kTile = kC * 128;     // bytes of a [128][64] 16-bit tile
 constexpr int kThreads = 20 * 32;
 constexpr int kWarpV = 4, kWarpS = 8, kWarpTma = 16, kWarpGate = 17, kWarpMma = 18, kWarpStore = 19;
 constexpr float kLog2e = 1.4426950408889634f;
-// a wait sleeps for up to this long at a time, and ends after so many cycles
-constexpr uint32_t kSleepNs = 20000, kWaitCycles = 2000u * 1000u * 1000u;
+constexpr uint32_t kWaitTries = 1u << 18;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
 // within this range e^(G_i - G_j) is taken as the product of e^G_i and e^-G_j
 constexpr float kNear = 100.f;
 
-// TMEM columns
+// TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
 constexpr uint32_t kTmQ = 128;    // Q' bf16 [DK / 2]
 constexpr uint32_t kTmV = 192;    // V'' [64]
@@ -76,21 +75,23 @@ struct Layout {
   static constexpr int kGate = kS + DK / 64 * kSBlock;
   static constexpr int kGateStage = 2 * kC * 4;            // G or e^-G, w
   static constexpr int kBars = kGate + 2 * kGateStage;
-  static constexpr int kBytes = kBars + 256;
+  static constexpr int kBytes = kBars + 320;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
+enum { kTileQ = 0, kTileK = 1, kTileV = 2 };
+
 struct Bars {
-  uint64_t full[2], empty_k[2], empty_v[2], empty_q[2];
+  uint64_t full[3][2], empty[3][2];  // of the Q, K, V tiles
   uint64_t gfull[2], gempty[2];
-  uint64_t sc_done, q_ready, qs_done, p_ready, pv_done;
-  uint64_t v_ready, v_free, ds_done, s_ready;
+  uint64_t sc_done, q_ready, q2_ready, qs_done, p_ready, pv_done;
+  uint64_t v_ready, v_free, ds_done, ds_free, s_ready;
   uint64_t o_free, o_staged, zeroed, drain;
   float gamma[2];
   int near_one[2];  // the chunk's e^G and e^-G both stay well inside fp32
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 256, "barriers");
+static_assert(sizeof(Bars) <= 320, "barriers");
 
 struct PrefillParams {
   lin_prefill_args_t a;
@@ -151,27 +152,45 @@ __device__ __forceinline__ float log2_gate(float g) {
   return x < kLowest ? kLowest : x;
 }
 
-// Waits for a phase, asleep in the barrier unit for most of it; false after about
-// a second.  Short on purpose: two dozen copies of it share the instruction cache
-// with the roles' loops.  wait1() is for one thread; wait() for a whole warp,
-// whose lanes all get the same answer.
+// Whether two phases are both complete: one look, asked for together.
+__device__ __forceinline__ bool both_done(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(b0)), "r"(p0), "r"(smem_u32(b1)), "r"(p1)
+      : "memory");
+  return ok != 0;
+}
+
+// Waits for a phase; false after about a second.  A try sleeps in the barrier unit
+// until the phase completes or 8000 cycles have gone by (measured; the hint makes no
+// difference), so the tries are what is counted: two dozen copies of this share the
+// instruction cache with the roles' loops, and no clock is read.  wait1() is for one
+// thread; wait() for a whole warp, whose lanes all get the same answer.
 __device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_u32(bar);
-  const uint32_t t0 = static_cast<uint32_t>(clock());
-  uint32_t ok;
+  uint32_t ok, tries = kWaitTries;
   do {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(at), "r"(parity), "r"(kSleepNs)
+        : "r"(at), "r"(parity)
         : "memory");
-  } while (!ok && static_cast<uint32_t>(clock()) - t0 < kWaitCycles);
+  } while (!ok && --tries);
   return ok != 0;
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
   return __all_sync(0xffffffffu, wait1(bar, parity));
+}
+__device__ __forceinline__ bool wait_both(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1) {
+  return __all_sync(0xffffffffu, both_done(b0, p0, b1, p1) || (wait1(b0, p0) && wait1(b1, p1)));
 }
 
 template <int DK, int BV, typename IO>
@@ -192,15 +211,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWarpMma) tc::tmem_alloc(&bar.tmem, 512);
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar.full[s], 1);
-      mbar_init(&bar.empty_k[s], 1);
-      mbar_init(&bar.empty_v[s], 1);
-      mbar_init(&bar.empty_q[s], 4);
+      for (int t = 0; t < 3; ++t) {
+        mbar_init(&bar.full[t][s], 1);
+        mbar_init(&bar.empty[t][s], t == kTileQ ? 4 : 1);
+      }
       mbar_init(&bar.gfull[s], 1);
       mbar_init(&bar.gempty[s], 16);
     }
     mbar_init(&bar.sc_done, 1);
     mbar_init(&bar.q_ready, 4);
+    mbar_init(&bar.q2_ready, 4);
+    mbar_init(&bar.ds_free, 8);
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
     mbar_init(&bar.pv_done, 1);
@@ -221,23 +242,21 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_wait();
   const Seq seq = find_seq(a, n, blockIdx.x == 0 && tid == 0);
   const int chunks = seq.len > 0 ? (seq.len + kC - 1) / kC : 0;
-  const uint32_t tmem = bar.tmem;
+  constexpr uint32_t tmem = 0;
   const uint32_t sb = smem_u32(smem);
   uint32_t* const status = a.status;
   bool ok = true;
 
   if (warp < kWarpV) {
-    // ------------------------------------------------ R: a row per thread
+    // ------------------------------------------------ R: P, a row per thread
     const int row = tid;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     for (int c = 0; c < chunks; ++c) {
       const int st = c & 1;
       const uint32_t ph = (c >> 1) & 1;
-      const unsigned char* stage = smem + st * L::kStage;
       const float* G = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage);
-      if (!(ok = wait(&bar.gfull[st], ph))) break;
-      if (!(ok = wait(&bar.full[st], ph))) break;
-      // the columns that the last chunk's QS has read
+      // Q into the columns that the last chunk's QS has read
+      if (!(ok = wait_both(&bar.gfull[st], ph, &bar.full[kTileQ][st], ph))) break;
       if (c && !(ok = wait(&bar.qs_done, (c - 1) & 1))) break;
       tc::fence_after_sync();
       const bool near_one = bar.near_one[st];
@@ -245,43 +264,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float f = a.scale * (near_one ? __frcp_rn(Gi) : ex2(Gi));
       const uint32_t f_hi = tc::pack2<true>(f, f);
       const uint32_t f_lo = tc::pack2<true>(f - tc::unpack_lo<true>(f_hi), f - tc::unpack_lo<true>(f_hi));
-      const auto put_q = [&](bool scaled) {
-#pragma unroll 1
-        for (int b = 0; b < DK / 64; ++b) {
-          uint32_t u[2][16];
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            lds128(stage + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
-          if (scaled) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              uint32_t& w = u[i >> 4][i & 15];
-              w = BF16 ? tc::fma2<true>(w, f_hi, tc::mul2<true>(w, f_lo))
-                       : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
-            }
-          }
-          tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
-          tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
-        }
-        tc::tmem_wait_st();
-      };
-      // bf16 near one: SC and QS both take Q'.  Else SC takes Q as it is, since
-      // e^G could leave the type's range, and Q' follows it.
+      // bf16 near one: SC and QS both take Q' = scale e^G Q.  Else SC takes Q as it
+      // is, since e^G could leave the type's range, and Q' (bf16) follows it.
       const bool shared_q = BF16 && near_one;
-      put_q(shared_q);
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.q_ready);
-
-      if (!(ok = wait(&bar.sc_done, c & 1))) break;
-      tc::fence_after_sync();
-      if (!shared_q) put_q(true);
-      tc::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bar.q_ready);
-        mbar_arrive(&bar.empty_q[st]);
+#pragma unroll 1
+      for (int pass = 0; pass < 2; ++pass) {
+        if (pass && !(ok = wait(&bar.sc_done, c & 1))) break;
+        tc::fence_after_sync();
+        if (!pass || !shared_q) {
+#pragma unroll 1
+          for (int b = 0; b < DK / 64; ++b) {
+            uint32_t u[2][16];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              lds128(smem + st * L::kStage + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
+            if (pass || shared_q) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                uint32_t& w = u[i >> 4][i & 15];
+                w = BF16 ? tc::fma2<true>(w, f_hi, tc::mul2<true>(w, f_lo))
+                         : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
+              }
+            }
+            tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
+            tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
+          }
+          tc::tmem_wait_st();
+          tc::fence_before_sync();
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(pass ? &bar.q2_ready : &bar.q_ready);
       }
+      if (!ok) break;
+      if (lane == 0) mbar_arrive(&bar.empty[kTileQ][st]);
       // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
 #pragma unroll 1
       for (int b = 0; b < 4; ++b) {
@@ -324,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp < kWarpS) {
-    // ------------------------------------------------ V: V'' parts
+    // ------------------------------------------------ V: V'' parts, O
     const int quarter = warp - kWarpV, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const bool has_rows = quarter * 32 < BV;
@@ -412,29 +427,29 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int step = 0; step <= 2 * chunks; ++step) {
       const int c = step >> 1, half = step & 1, st = c & 1;
       if (c < chunks) {
-      if (half == 0) {
-        const uint32_t ph = (c >> 1) & 1;
-        if (!(ok = wait(&bar.gfull[st], ph))) break;
-        if (!(ok = wait(&bar.full[st], ph))) break;
-        const int rows = seq.len - c * kC;
-        if (rows < kC) {
-          // rows of the next sequence, or outside: zero, whatever they hold, since
-          // 0 x NaN would reach the sums over the chunk's tokens
-          unsigned char* stage = smem + st * L::kStage;
-          for (int r = rows + quarter; r < kC; r += 4)
-            for (int i = lane; i < (DK + BV) / 8; i += 32)
-              *reinterpret_cast<uint4*>(stage + L::kK + (i >> 3) * kTile + tc::sw128_offset(r, i & 7)) =
-                  make_uint4(0, 0, 0, 0);
-          tc::fence_proxy_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bar.zeroed);
-          if (!(ok = wait(&bar.zeroed, 0))) break;  // only the last chunk is short
+        if (half == 0) {
+          const uint32_t ph = (c >> 1) & 1;
+          if (!(ok = wait_both(&bar.gfull[st], ph, &bar.full[kTileV][st], ph))) break;
+          const int rows = seq.len - c * kC;
+          if (rows < kC) {
+            // rows of the next sequence, or outside: zero, whatever they hold, since
+            // 0 x NaN would reach the sums over the chunk's tokens
+            if (!(ok = wait(&bar.full[kTileK][st], ph))) break;
+            unsigned char* stage = smem + st * L::kStage;
+            for (int r = rows + quarter; r < kC; r += 4)
+              for (int i = lane; i < (DK + BV) / 8; i += 32)
+                *reinterpret_cast<uint4*>(stage + L::kK + (i >> 3) * kTile + tc::sw128_offset(r, i & 7)) =
+                    make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bar.zeroed);
+            if (!(ok = wait(&bar.zeroed, 0))) break;  // only the last chunk is short
+          }
         }
-      }
-      if (step && !(ok = wait(&bar.v_free, half ^ 1))) break;
-      tc::fence_after_sync();
-      parts(c, half);
-      if (half && lane == 0) mbar_arrive(&bar.gempty[st]);
+        if (step && !(ok = wait(&bar.v_free, half ^ 1))) break;
+        tc::fence_after_sync();
+        parts(c, half);
+        if (half && lane == 0) mbar_arrive(&bar.gempty[st]);
       }
       if (c && !half && !(ok = output(c - 1))) break;
     }
@@ -456,12 +471,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int c = -1; c < chunks; ++c) {
       if (c >= 0) {
         const int st = c & 1;
-        ok = wait(&bar.gfull[st], (c >> 1) & 1) && wait(&bar.ds_done, c & 1);
+        ok = wait_both(&bar.gfull[st], (c >> 1) & 1, &bar.ds_done, c & 1);
         if (!ok) break;
         tc::fence_after_sync();
         const float gamma = bar.gamma[st];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bar.gempty[st]);
         if (has_rows) {
 #pragma unroll
           for (int b = 0; b < kN / 16; ++b) {
@@ -471,6 +484,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], d[e]);
           }
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.gempty[st]);
+          mbar_arrive(&bar.ds_free);
         }
       }
       if (has_rows) {  // S^T rounded to bf16, the QS product's operand
@@ -482,7 +501,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                      tc::pack2<true>(S[8 * i + 4], S[8 * i + 5]), tc::pack2<true>(S[8 * i + 6], S[8 * i + 7]));
         }
       }
-      tc::fence_before_sync();
       tc::fence_proxy_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.s_ready);
@@ -493,44 +511,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < kN; ++i) to[static_cast<int64_t>(i) * a.dv] = S[i];
     }
   } else if (warp == kWarpTma) {
-    if (lane == 0) {
-      int c = 0;
-      for (; c < chunks; ++c) {
+    if (tc::elect_one()) {
+      // in the order in which the tiles come free; a tile's barrier is armed only
+      // then, when its last load is known to be complete
+      int armed[3] = {0, 0, 0};
+      for (int c = 0; c < chunks && ok; ++c) {
         const int st = c & 1;
         unsigned char* stage = smem + st * L::kStage;
         const int t = seq.start + c * kC;
-        const uint32_t ph = ((c >> 1) & 1) ^ 1;
-        // In the order in which the tiles come free.  The barrier is armed for the
-        // stage only once its Q tile is free, and so the chunk before complete.
-        if (c >= 2 && !(ok = wait1(&bar.empty_q[st], ph))) break;
-        mbar_arrive_expect_tx(&bar.full[st], L::kStage);
-        for (int b = 0; b < DK / 64; ++b) tc::tma_load_4d(stage + L::kQ + b * kTile, &map_q, b * 64, hq, t, batch, &bar.full[st]);
-        uint32_t missing = (DK + BV) / 64 * kTile;
-        if (c < 2 || wait1(&bar.empty_v[st], ph)) {
-          for (int b = 0; b < BV / 64; ++b)
-            tc::tma_load_4d(stage + L::kV + b * kTile, &map_v, vb * BV + b * 64, h, t, batch, &bar.full[st]);
-          missing -= BV / 64 * kTile;
-          if (c < 2 || wait1(&bar.empty_k[st], ph)) {
-            for (int b = 0; b < DK / 64; ++b)
-              tc::tma_load_4d(stage + L::kK + b * kTile, &map_k, b * 64, hq, t, batch, &bar.full[st]);
-            missing = 0;
-          }
-        }
-        if (missing) {  // given up: the drain below ends on what was issued
-          asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(&bar.full[st])),
-                       "r"(missing)
-                       : "memory");
-          ok = false;
-          ++c;
-          break;
-        }
+        const auto load = [&](int tile, const CUtensorMap* map, int at, int blocks, int x, int head) {
+          if (c >= 2 && !wait1(&bar.empty[tile][st], ((c >> 1) & 1) ^ 1)) return false;
+          mbar_arrive_expect_tx(&bar.full[tile][st], blocks * kTile);
+          for (int b = 0; b < blocks; ++b)
+            tc::tma_load_4d(stage + at + b * kTile, map, x + b * 64, head, t, batch, &bar.full[tile][st]);
+          armed[tile] = c + 1;
+          return true;
+        };
+        ok = load(kTileQ, &map_q, L::kQ, DK / 64, 0, hq) && load(kTileV, &map_v, L::kV, BV / 64, vb * BV, h) &&
+             load(kTileK, &map_k, L::kK, DK / 64, 0, hq);
       }
       // no copy may be in flight when the shared memory is released
-      for (int j = max(0, c - 2); j < c; ++j)
-        if (!wait1(&bar.full[j & 1], (j >> 1) & 1)) {
-          ok = false;
-          break;
-        }
+#pragma unroll
+      for (int tile = 0; tile < 3; ++tile)
+        for (int j = max(0, armed[tile] - 2); j < armed[tile]; ++j)
+          if (!wait1(&bar.full[tile][j & 1], (j >> 1) & 1)) ok = false;
     }
   } else if (warp == kWarpGate) {
     // ------------------------------------------------ gates: 4 tokens per lane
@@ -547,25 +551,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (c < 0) continue;
       const int st = c & 1;
       float* G = reinterpret_cast<float*>(smem + L::kGate + st * L::kGateStage);
-      // cumulative in fp64: differences of far sums keep their small part
-      double s[4];
-      s[0] = log2_gate(x[0]);
+      // G summed from the front; the weights' exponents from the back, so that those
+      // near zero are sums of few small numbers and keep their precision
+      float fwd[4], bwd[4];
+      fwd[0] = x[0] = log2_gate(x[0]);
 #pragma unroll
-      for (int e = 1; e < 4; ++e) s[e] = s[e - 1] + static_cast<double>(log2_gate(x[e]));
-      double inc = s[3];
+      for (int e = 1; e < 4; ++e) fwd[e] = fwd[e - 1] + (x[e] = log2_gate(x[e]));
+      bwd[3] = 0.f;
+#pragma unroll
+      for (int e = 2; e >= 0; --e) bwd[e] = bwd[e + 1] + x[e + 1];
+      float before = fwd[3], after = fwd[3];
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
-        const double y = __shfl_up_sync(0xffffffffu, inc, off);
-        if (lane >= off) inc += y;
+        const float y = __shfl_up_sync(0xffffffffu, before, off), z = __shfl_down_sync(0xffffffffu, after, off);
+        if (lane >= off) before += y;
+        if (lane + off < 32) after += z;
       }
-      const double before = inc - s[3], end = __shfl_sync(0xffffffffu, inc, 31);
+      const float end = __shfl_sync(0xffffffffu, before, 31);
+      before = __shfl_up_sync(0xffffffffu, before, 1);
+      after = __shfl_down_sync(0xffffffffu, after, 1);
+      if (lane == 0) before = 0.f;
+      if (lane == 31) after = 0.f;
       if (c >= 2 && !(ok = wait(&bar.gempty[st], ((c >> 1) & 1) ^ 1))) break;
       float far = 0.f, gv[4], wv[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const double Gt = before + s[e];
-        gv[e] = static_cast<float>(Gt);
-        wv[e] = c * kC + lane * 4 + e < seq.len ? ex2(static_cast<float>(end - Gt)) : 0.f;
+        gv[e] = before + fwd[e];
+        wv[e] = c * kC + lane * 4 + e < seq.len ? ex2(after + bwd[e]) : 0.f;
         far = fmaxf(far, fabsf(gv[e]));
       }
       const bool near_one = __all_sync(0xffffffffu, far <= kNear);
@@ -583,14 +595,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       *reinterpret_cast<uint4*>(G + kC + lane * 4) = make_uint4(wp[0], wp[1], wp[2], wp[3]);
       if (lane == 0) {
-        bar.gamma[st] = ex2(static_cast<float>(end));
+        bar.gamma[st] = ex2(end);
         bar.near_one[st] = near_one;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.gfull[st]);
     }
   } else if (warp == kWarpStore) {
-    if (lane == 0) {  // whole chunks of O leave by TMA; V writes a short one
+    if (tc::elect_one()) {  // whole chunks of O leave by TMA; V writes a short one
       for (int c = 0; c < chunks && seq.len - c * kC >= kC; ++c) {
         const int st = c & 1;
         if (!(ok = wait1(&bar.o_staged, c & 1))) break;
@@ -598,17 +610,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::tma_store_4d(&map_o, smem + st * L::kStage + L::kO + b * kTile, vb * BV + b * 64, h, seq.start + c * kC, batch);
         bulk_commit();
         bulk_wait_read();
-        mbar_arrive(L::kOInK ? &bar.empty_k[st] : &bar.empty_v[st]);
+        mbar_arrive(L::kOInK ? &bar.empty[kTileK][st] : &bar.empty[kTileV][st]);
       }
       bulk_wait_all();
     }
-  } else if (warp == kWarpMma && lane == 0) {
+  } else if (warp == kWarpMma && tc::elect_one()) {
     // ------------------------------------------------ MMA
     constexpr uint32_t kIdSC = tc::idesc_f16(128, kC, false, false, BF16);
     constexpr uint32_t kIdDS = tc::idesc_f16(128, DK, false, true, BF16);
     constexpr uint32_t kIdQS = tc::idesc_f16(128, BV, false, false, true);
     constexpr uint32_t kIdPV = tc::idesc_f16(128, BV, false, true, BF16);
-        for (int c = 0; c < chunks; ++c) {
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
       const int st = c & 1;
       // step s of an operand lies a constant number of 16-byte units after step 0
       const uint32_t stage = sb + st * L::kStage;
@@ -617,34 +630,31 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint64_t sT = tc::kmajor_desc(sb + L::kS, L::kSBlock, 0);
       const auto along = [](int s, int block) { return static_cast<uint64_t>(((s >> 2) * block + (s & 3) * 32) >> 4); };
       const auto add_ds = [&](int half) {  // 64 tokens: the small parts, then the large ones
-#pragma unroll 2
+#pragma unroll
         for (int s = 0; s < 8; ++s)
-          tc::mma_tmem_a(tmem + kTmDS, tmem + kTmV + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
+          tc::mma_tmem_a(kTmDS, kTmV + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
       };
-      ok = wait1(&bar.full[st], (c >> 1) & 1) &&
-           wait1(&bar.q_ready, 0) &&
+      ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1) && wait1(&bar.q_ready, c & 1) &&
            (c == 0 || wait1(&bar.pv_done, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll 2
+#pragma unroll
       for (int s = 0; s < DK / 16; ++s)
-        tc::mma_tmem_a(tmem + kTmSC, tmem + kTmQ + s * 8, k + along(s, kTile), kIdSC, s > 0);
+        tc::mma_tmem_a(kTmSC, kTmQ + s * 8, k + along(s, kTile), kIdSC, s > 0);
       tc::commit(&bar.sc_done);
 
-      ok = wait1(&bar.s_ready, c & 1) &&
-           wait1(&bar.v_ready, 0);
+      ok = wait1(&bar.v_ready, 0) && (c == 0 || wait1(&bar.ds_free, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
       add_ds(0);
       tc::commit(&bar.v_free);
 
-      ok = wait1(&bar.q_ready, 1) &&
-           (c == 0 || wait1(&bar.o_free, (c - 1) & 1));
+      ok = wait1(&bar.q2_ready, c & 1) && wait1(&bar.s_ready, c & 1) && (c == 0 || wait1(&bar.o_free, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll 2
+#pragma unroll
       for (int s = 0; s < DK / 16; ++s)
-        tc::mma_tmem_a(tmem + kTmO, tmem + kTmQ + s * 8, sT + along(s, L::kSBlock), kIdQS, s > 0);
+        tc::mma_tmem_a(kTmO, kTmQ + s * 8, sT + along(s, L::kSBlock), kIdQS, s > 0);
       tc::commit(&bar.qs_done);
 
       ok = wait1(&bar.v_ready, 1);
@@ -657,11 +667,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       ok = wait1(&bar.p_ready, c & 1);
       if (!ok) break;
       tc::fence_after_sync();
-#pragma unroll 2
+#pragma unroll
       for (int s = 0; s < kC / 16; ++s)
-        tc::mma_tmem_a(tmem + kTmO, tmem + kTmSC + s * 8, v + s * 128, kIdPV, true);
+        tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
       tc::commit(&bar.pv_done);
-      tc::commit(L::kOInK ? &bar.empty_v[st] : &bar.empty_k[st]);
+      tc::commit(L::kOInK ? &bar.empty[kTileV][st] : &bar.empty[kTileK][st]);
     }
     if (!ok) {  // products in flight end before the tensor memory is released
       tc::commit(&bar.drain);

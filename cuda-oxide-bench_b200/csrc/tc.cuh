@@ -162,6 +162,19 @@ __device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// True in one lane of a converged warp.  The compiler knows the instruction: in
+// code under it, tcgen05 and TMA operands go straight to uniform registers, where
+// under a test of the lane number each issue carries a sequence for many lanes.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
+
 // Named barrier over `count` threads (a thread group inside the CTA).
 __device__ __forceinline__ void group_sync(int id, int count) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(count) : "memory");
