@@ -85,7 +85,7 @@ struct Bars {
   uint64_t full[3][2], empty[3][2];  // of the Q, K, V tiles
   uint64_t gfull[2], gempty[2];
   uint64_t sc_done, q_ready, q2_ready, qs_done, p_ready, pv_done;
-  uint64_t v_ready, v_free, ds_done, ds_free, s_ready;
+  uint64_t v_ready[2], v_free[2], ds_done, ds_free, s_ready;
   uint64_t o_free, o_staged, zeroed, drain;
   float gamma[2];
   int near_one[2];  // the chunk's e^G and e^-G both stay well inside fp32
@@ -96,26 +96,44 @@ static_assert(sizeof(Bars) <= 320, "barriers");
 struct PrefillParams {
   lin_prefill_args_t a;
   int nvb;
+  // Few rows and a long time axis: sequences of more than `piece` tokens are cut
+  // into pieces (0: none is).  A slot of the workspace per piece of a cut sequence
+  // holds the state that the piece starts from, and first the piece before's own
+  // contribution; `decay` the pieces' products of gates, [slot][head].
+  int piece, pieces, slots;  // pieces: of every sequence, in the dense form
+  float* slot_state;
+  float* decay;
 };
 
-// Where sequence n lies: first row, tokens, page (-1: none).
+// What a CTA works on: `len` tokens from row `start` (-1: nothing), beginning with
+// the state `from` (NULL: zero) and leaving it in `to` (NULL: nowhere).
+struct Item {
+  int start, len;
+  const float* from;
+  float* to;
+};
+
 struct Seq {
   int start, len, page;
 };
 
-// Every thread of the CTA calls it.  Offsets out of range or descending give a
-// sequence of -1 tokens; a page out of range or held by an earlier sequence none.
-__device__ Seq find_seq(const lin_prefill_args_t& a, int n, bool reporter) {
-  Seq s;
+// Sequence n's rows; offsets out of range or descending give -1 tokens.
+__device__ __forceinline__ void find_rows(const lin_prefill_args_t& a, int n, Seq& s) {
   s.start = 0;
   s.len = a.T;
-  bool bad = false;
   if (a.cu_seqlens) {
     const int lo = a.cu_seqlens[n], hi = a.cu_seqlens[n + 1];
-    bad = !(lo >= 0 && lo <= hi && hi <= a.T);
     s.start = lo;
-    s.len = bad ? -1 : hi - lo;
+    s.len = lo >= 0 && lo <= hi && hi <= a.T ? hi - lo : -1;
   }
+}
+
+// Every thread of the CTA calls it.  A page out of range or held by an earlier
+// sequence is none (-1).
+__device__ Seq find_seq(const lin_prefill_args_t& a, int n, bool reporter) {
+  Seq s;
+  find_rows(a, n, s);
+  bool bad = s.len < 0;
   s.page = a.index ? a.index[n] : n;
   bool taken = s.page >= a.pages;
   if (a.index && s.page >= 0)
@@ -126,6 +144,84 @@ __device__ Seq find_seq(const lin_prefill_args_t& a, int n, bool reporter) {
   }
   if (bad && reporter) report(a.status, GDN_DEVERR_BAD_INDEX);
   return s;
+}
+
+// Slots of sequence n: one per piece if it is cut.
+__device__ __forceinline__ int slots_of(const PrefillParams& p, int n) {
+  if (n >= p.a.B) return 0;
+  Seq s;
+  find_rows(p.a, n, s);
+  return s.len > p.piece ? (s.len + p.piece - 1) / p.piece : 0;
+}
+
+// Whole warps: the sequence that slot y belongs to (-1: none) and the piece, or,
+// with y < 0, the first slot of sequence *n.
+__device__ int find_slot(const PrefillParams& p, int y, int* n) {
+  if (!p.a.cu_seqlens) {
+    if (y < 0) return *n * p.pieces;
+    *n = y / p.pieces;
+    return y - *n * p.pieces;
+  }
+  const int lane = threadIdx.x & 31;
+  const int until = y < 0 ? *n : p.a.B;
+  int run = 0;
+  for (int n0 = 0; n0 < until; n0 += 32) {
+    const int v = n0 + lane < until ? slots_of(p, n0 + lane) : 0;
+    int inc = v;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += x;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, y >= 0 && y < run + inc);
+    if (past) {
+      const int hit = __ffs(past) - 1;
+      *n = n0 + hit;
+      return y - run - __shfl_sync(0xffffffffu, inc - v, hit);
+    }
+    run += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (y < 0) return run;
+  *n = -1;
+  return 0;
+}
+
+template <bool FULL>
+__device__ Item find_item(const PrefillParams& p, int y, bool reporter) {
+  const lin_prefill_args_t& a = p.a;
+  const int64_t page = static_cast<int64_t>(a.Hv) * a.dk * a.dv;
+  Item it{0, -1, nullptr, nullptr};
+  int n = y, at = 0;
+  const bool slot = p.piece && y < p.slots;
+  if (slot) {
+    at = find_slot(p, y, &n);
+    if (n < 0) return it;
+  } else if (p.piece) {
+    n = y - p.slots;
+  }
+  const Seq s = find_seq(a, n, reporter);
+  if (s.len < 0) return it;
+  const bool cut = p.piece && s.len > p.piece;
+  if (!slot) {
+    if (cut) return it;
+    it.start = s.start;
+    it.len = s.len;
+    if (s.page >= 0 && a.initial_state) it.from = a.initial_state + s.page * a.initial_sp;
+    if (s.page >= 0) it.to = a.final_state + s.page * a.final_sp;
+    return it;
+  }
+  const bool last = (at + 1) * p.piece >= s.len;
+  // (overlapping sequences, which unsound offsets allow, could ask for more slots)
+  if (!FULL && (last || y + 1 >= p.slots)) return it;
+  it.start = s.start + at * p.piece;
+  it.len = last ? s.len - at * p.piece : p.piece;
+  if (FULL) {
+    it.from = p.slot_state + y * page;
+    if (last && s.page >= 0) it.to = a.final_state + s.page * a.final_sp;
+  } else {
+    it.to = p.slot_state + (y + 1) * page;
+  }
+  return it;
 }
 
 // Shared-memory loads that stay where they are written: ahead of the arithmetic.
@@ -193,7 +289,9 @@ __device__ __forceinline__ bool wait_both(uint64_t* b0, uint32_t p0, uint64_t* b
   return __all_sync(0xffffffffu, both_done(b0, p0, b1, p1) || (wait1(b0, p0) && wait1(b1, p1)));
 }
 
-template <int DK, int BV, typename IO>
+// FULL: everything.  Else only what a piece adds to the state and its decay, from k,
+// v and the gates; the tensor memory that is free then is a second place for V''.
+template <int DK, int BV, typename IO, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1)
     lin_prefill_kernel(const __grid_constant__ PrefillParams p, const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -205,8 +303,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const lin_prefill_args_t& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.x / p.nvb, vb = blockIdx.x - h * p.nvb, hq = h / (a.Hv / a.Hqk);
-  const int n = blockIdx.y;
-  const int batch = a.cu_seqlens ? 0 : n;
+  pdl_launch_dependents();
+  pdl_wait();
+  const Item seq = find_item<FULL>(p, blockIdx.y, FULL && blockIdx.x == 0 && tid == 0);
+  if (seq.len < 0) return;
+  const int chunks = (seq.len + kC - 1) / kC;
+  const int batch = a.cu_seqlens ? 0 : p.piece && static_cast<int>(blockIdx.y) < p.slots ? blockIdx.y / p.pieces
+                                    : blockIdx.y - (p.piece ? p.slots : 0);
 
   if (warp == kWarpMma) tc::tmem_alloc(&bar.tmem, 512);
   if (tid == 0) {
@@ -216,7 +319,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&bar.empty[t][s], t == kTileQ ? 4 : 1);
       }
       mbar_init(&bar.gfull[s], 1);
-      mbar_init(&bar.gempty[s], 16);
+      mbar_init(&bar.gempty[s], FULL ? 16 : 12);
+      mbar_init(&bar.v_ready[s], 4);
+      mbar_init(&bar.v_free[s], 1);
     }
     mbar_init(&bar.sc_done, 1);
     mbar_init(&bar.q_ready, 4);
@@ -225,8 +330,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
     mbar_init(&bar.pv_done, 1);
-    mbar_init(&bar.v_ready, 4);
-    mbar_init(&bar.v_free, 1);
     mbar_init(&bar.ds_done, 1);
     mbar_init(&bar.s_ready, 8);
     mbar_init(&bar.o_free, 4);
@@ -235,19 +338,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
   }
-  pdl_launch_dependents();
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
-  pdl_wait();
-  const Seq seq = find_seq(a, n, blockIdx.x == 0 && tid == 0);
-  const int chunks = seq.len > 0 ? (seq.len + kC - 1) / kC : 0;
   constexpr uint32_t tmem = 0;
   const uint32_t sb = smem_u32(smem);
   uint32_t* const status = a.status;
   bool ok = true;
 
-  if (warp < kWarpV) {
+  if (FULL && warp < kWarpV) {
     // ------------------------------------------------ R: P, a row per thread
     const int row = tid;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
@@ -338,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bar.gempty[st]);
       }
     }
-  } else if (warp < kWarpS) {
+  } else if (warp >= kWarpV && warp < kWarpS) {
     // ------------------------------------------------ V: V'' parts, O
     const int quarter = warp - kWarpV, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -370,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             hi[e] = tc::fma2<BF16>(v, w_hi, tc::mul2<BF16>(v, w_lo));
             lo[e] = tc::fma2<BF16>(v, w_lo, tc::fma2<BF16>(v, w_hi, hi[e] ^ 0x80008000u));
           }
-          const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + kTmV;
+          const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + (FULL || half ? kTmV : kTmSC);
           tc::tmem_st_16x128b_x8(to, lo);
           tc::tmem_st_16x128b_x8(to + 32, hi);
         }
@@ -378,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tc::fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar.v_ready);
+      if (lane == 0) mbar_arrive(&bar.v_ready[half]);
     };
     // O of chunk c: a token per thread, packed into shared memory
     const auto output = [&](int c) {
@@ -424,7 +523,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Two steps a chunk, 64 tokens each, the last chunk's output between them.
     // One call site each keeps the kernel's code within the instruction cache.
 #pragma unroll 1
-    for (int step = 0; step <= 2 * chunks; ++step) {
+    for (int step = 0; step < 2 * chunks + FULL; ++step) {
       const int c = step >> 1, half = step & 1, st = c & 1;
       if (c < chunks) {
         if (half == 0) {
@@ -446,14 +545,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = wait(&bar.zeroed, 0))) break;  // only the last chunk is short
           }
         }
-        if (step && !(ok = wait(&bar.v_free, half ^ 1))) break;
+        // the columns' last user: the half before, or this half of the chunk before
+        const int before = FULL ? step - 1 : step - 2;
+        if (before >= 0 && !(ok = wait(&bar.v_free[before & 1], (before >> 1) & 1))) break;
         tc::fence_after_sync();
         parts(c, half);
         if (half && lane == 0) mbar_arrive(&bar.gempty[st]);
       }
-      if (c && !half && !(ok = output(c - 1))) break;
+      if (FULL && c && !half && !(ok = output(c - 1))) break;
     }
-  } else if (warp < kWarpTma) {
+  } else if (warp >= kWarpS && warp < kWarpTma) {
     // ------------------------------------------------ S: the state, a value column per thread
     const int quarter = warp & 3, half = (warp - kWarpS) >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -462,13 +563,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr int kN = DK / 2;            // d_k entries of this thread
     const int64_t at = (static_cast<int64_t>(h) * DK + half * kN) * a.dv + vb * BV + row;
     float S[kN];
-    const bool load = has_rows && seq.page >= 0 && a.initial_state && seq.len >= 0;
-    const float* from = a.initial_state + (load ? seq.page * a.initial_sp + at : 0);
+    const float* from = seq.from + (seq.from ? at : 0);
 #pragma unroll
-    for (int i = 0; i < kN; ++i) S[i] = load ? from[static_cast<int64_t>(i) * a.dv] : 0.f;
+    for (int i = 0; i < kN; ++i) S[i] = seq.from && has_rows ? from[static_cast<int64_t>(i) * a.dv] : 0.f;
     // the state before chunk 0, then after each chunk
 #pragma unroll 1
-    for (int c = -1; c < chunks; ++c) {
+    for (int c = FULL ? -1 : 0; c < chunks; ++c) {
       if (c >= 0) {
         const int st = c & 1;
         ok = wait_both(&bar.gfull[st], (c >> 1) & 1, &bar.ds_done, c & 1);
@@ -492,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bar.ds_free);
         }
       }
+      if (!FULL) continue;
       if (has_rows) {  // S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
@@ -505,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.s_ready);
     }
-    if (ok && has_rows && seq.page >= 0 && seq.len >= 0) {
-      float* to = a.final_state + seq.page * a.final_sp + at;
+    if (ok && has_rows && seq.to) {
+      float* to = seq.to + at;
 #pragma unroll
       for (int i = 0; i < kN; ++i) to[static_cast<int64_t>(i) * a.dv] = S[i];
     }
@@ -527,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           armed[tile] = c + 1;
           return true;
         };
-        ok = load(kTileQ, &map_q, L::kQ, DK / 64, 0, hq) && load(kTileV, &map_v, L::kV, BV / 64, vb * BV, h) &&
+        ok = (!FULL || load(kTileQ, &map_q, L::kQ, DK / 64, 0, hq)) && load(kTileV, &map_v, L::kV, BV / 64, vb * BV, h) &&
              load(kTileK, &map_k, L::kK, DK / 64, 0, hq);
       }
       // no copy may be in flight when the shared memory is released
@@ -539,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kWarpGate) {
     // ------------------------------------------------ gates: 4 tokens per lane
     const int64_t g0 = batch * a.g_sb + h * a.g_sh;
-    float x[4], next[4];
+    float x[4], next[4], sum = 0.f;
 #pragma unroll 1
     for (int c = -1; c < chunks; ++c) {  // a chunk's gates are fetched while the one before is at work
 #pragma unroll
@@ -568,6 +669,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane + off < 32) after += z;
       }
       const float end = __shfl_sync(0xffffffffu, before, 31);
+      sum += end;
       before = __shfl_up_sync(0xffffffffu, before, 1);
       after = __shfl_down_sync(0xffffffffu, after, 1);
       if (lane == 0) before = 0.f;
@@ -601,7 +703,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.gfull[st]);
     }
-  } else if (warp == kWarpStore) {
+    if (!FULL && lane == 0 && vb == 0) p.decay[static_cast<int64_t>(blockIdx.y) * a.Hv + h] = ex2(sum);
+  } else if (FULL && warp == kWarpStore) {
     if (tc::elect_one()) {  // whole chunks of O leave by TMA; V writes a short one
       for (int c = 0; c < chunks && seq.len - c * kC >= kC; ++c) {
         const int st = c & 1;
@@ -632,46 +735,56 @@ __global__ void __launch_bounds__(kThreads, 1)
       const auto add_ds = [&](int half) {  // 64 tokens: the small parts, then the large ones
 #pragma unroll
         for (int s = 0; s < 8; ++s)
-          tc::mma_tmem_a(kTmDS, kTmV + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
+          tc::mma_tmem_a(kTmDS, (FULL || half ? kTmV : kTmSC) + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
       };
-      ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1) && wait1(&bar.q_ready, c & 1) &&
-           (c == 0 || wait1(&bar.pv_done, (c - 1) & 1));
-      if (!ok) break;
-      tc::fence_after_sync();
+      if constexpr (FULL) {
+        ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1) && wait1(&bar.q_ready, c & 1) &&
+             (c == 0 || wait1(&bar.pv_done, (c - 1) & 1));
+        if (!ok) break;
+        tc::fence_after_sync();
 #pragma unroll
-      for (int s = 0; s < DK / 16; ++s)
-        tc::mma_tmem_a(kTmSC, kTmQ + s * 8, k + along(s, kTile), kIdSC, s > 0);
-      tc::commit(&bar.sc_done);
+        for (int s = 0; s < DK / 16; ++s)
+          tc::mma_tmem_a(kTmSC, kTmQ + s * 8, k + along(s, kTile), kIdSC, s > 0);
+        tc::commit(&bar.sc_done);
+      }
 
-      ok = wait1(&bar.v_ready, 0) && (c == 0 || wait1(&bar.ds_free, (c - 1) & 1));
+      ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1) && wait1(&bar.v_ready[0], c & 1) &&
+           (c == 0 || wait1(&bar.ds_free, (c - 1) & 1));
       if (!ok) break;
       tc::fence_after_sync();
       add_ds(0);
-      tc::commit(&bar.v_free);
+      tc::commit(&bar.v_free[0]);
 
-      ok = wait1(&bar.q2_ready, c & 1) && wait1(&bar.s_ready, c & 1) && (c == 0 || wait1(&bar.o_free, (c - 1) & 1));
-      if (!ok) break;
-      tc::fence_after_sync();
+      if constexpr (FULL) {
+        ok = wait1(&bar.q2_ready, c & 1) && wait1(&bar.s_ready, c & 1) && (c == 0 || wait1(&bar.o_free, (c - 1) & 1));
+        if (!ok) break;
+        tc::fence_after_sync();
 #pragma unroll
-      for (int s = 0; s < DK / 16; ++s)
-        tc::mma_tmem_a(kTmO, kTmQ + s * 8, sT + along(s, L::kSBlock), kIdQS, s > 0);
-      tc::commit(&bar.qs_done);
+        for (int s = 0; s < DK / 16; ++s)
+          tc::mma_tmem_a(kTmO, kTmQ + s * 8, sT + along(s, L::kSBlock), kIdQS, s > 0);
+        tc::commit(&bar.qs_done);
+      }
 
-      ok = wait1(&bar.v_ready, 1);
+      ok = wait1(&bar.v_ready[1], c & 1);
       if (!ok) break;
       tc::fence_after_sync();
       add_ds(1);
-      tc::commit(&bar.v_free);
+      tc::commit(&bar.v_free[1]);
       tc::commit(&bar.ds_done);
 
-      ok = wait1(&bar.p_ready, c & 1);
-      if (!ok) break;
-      tc::fence_after_sync();
+      if constexpr (FULL) {
+        ok = wait1(&bar.p_ready, c & 1);
+        if (!ok) break;
+        tc::fence_after_sync();
 #pragma unroll
-      for (int s = 0; s < kC / 16; ++s)
-        tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
-      tc::commit(&bar.pv_done);
-      tc::commit(L::kOInK ? &bar.empty[kTileV][st] : &bar.empty[kTileK][st]);
+        for (int s = 0; s < kC / 16; ++s)
+          tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
+        tc::commit(&bar.pv_done);
+        tc::commit(L::kOInK ? &bar.empty[kTileV][st] : &bar.empty[kTileK][st]);
+      } else {
+        tc::commit(&bar.empty[kTileV][st]);
+        tc::commit(&bar.empty[kTileK][st]);
+      }
     }
     if (!ok) {  // products in flight end before the tensor memory is released
       tc::commit(&bar.drain);
@@ -686,6 +799,36 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == kWarpMma) tc::tmem_dealloc(tmem, 512);
 }
 
+// The states that the pieces of cut sequences start from: slot j + 1 holds what
+// piece j adds, and gets decay_j (slot j) + that; slot 0 the initial state.
+__global__ void __launch_bounds__(256) lin_scan_kernel(const __grid_constant__ PrefillParams p) {
+  const lin_prefill_args_t& a = p.a;
+  pdl_launch_dependents();
+  pdl_wait();
+  int n = blockIdx.y;
+  const int count = slots_of(p, n);
+  if (!count) return;
+  const int first = find_slot(p, -1, &n);
+  if (first + count > p.slots) return;
+  const Seq s = find_seq(a, n, false);
+  const int64_t page = static_cast<int64_t>(a.Hv) * a.dk * a.dv;
+  const int64_t e = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  if (e >= page) return;
+  const int h = static_cast<int>(e / (static_cast<int64_t>(a.dk) * a.dv));
+  float4 S = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (s.page >= 0 && a.initial_state)
+    S = *reinterpret_cast<const float4*>(a.initial_state + s.page * a.initial_sp + e);
+  float* slot = p.slot_state + first * page + e;
+  *reinterpret_cast<float4*>(slot) = S;
+  for (int j = 0; j + 1 < count; ++j) {
+    slot += page;
+    const float4 x = *reinterpret_cast<const float4*>(slot);
+    const float d = p.decay[static_cast<int64_t>(first + j) * a.Hv + h];
+    S = make_float4(fmaf(d, S.x, x.x), fmaf(d, S.y, x.y), fmaf(d, S.z, x.z), fmaf(d, S.w, x.w));
+    *reinterpret_cast<float4*>(slot) = S;
+  }
+}
+
 int io_map(CUtensorMap* m, bool bf16, const void* base, int d, int heads, int T, int B, int64_t sh, int64_t st, int64_t sb) {
   const uint64_t dims[4] = {static_cast<uint64_t>(d), static_cast<uint64_t>(heads), static_cast<uint64_t>(T),
                             static_cast<uint64_t>(B)};
@@ -697,14 +840,82 @@ int io_map(CUtensorMap* m, bool bf16, const void* base, int d, int heads, int T,
                     box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+template <typename... Args>
+int launch_pdl(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}
+
+// How the time axis is cut, and the workspace that takes.
+struct Cut {
+  int piece = 0, pieces = 0;
+  int64_t slots = 0, state_bytes = 0, bytes = 0;
+};
+
+int block_cols(const lin_prefill_args_t& a) { return a.dv % 128 == 0 ? 128 : 64; }
+
+Cut choose_cut(const lin_prefill_args_t& a, int sms) {
+  Cut cut;
+  const int64_t rows = static_cast<int64_t>(a.Hv) * (a.dv / block_cols(a));  // CTAs of one sequence
+  const int64_t chunks = (static_cast<int64_t>(a.T) + kC - 1) / kC;
+  if (a.cu_seqlens) {
+    // Lengths are known on the device only: cut what would keep its CTAs busy for
+    // more than half of the time that the whole work takes, and 2048 tokens at least.
+    const int64_t share = (chunks * rows + 2 * sms - 1) / (2 * sms);
+    const int64_t most = share > 16 ? share : 16;
+    if (chunks < 4 * most) return cut;
+    cut.piece = static_cast<int>(most * kC);
+    cut.slots = 2 * (static_cast<int64_t>(a.T) / cut.piece);
+  } else {
+    // Cost in chunks of time, kStart of them to start a CTA, a piece's state pass
+    // kState of a whole one, kScan for the scan and the launches (measured, d = 128).
+    constexpr double kStart = 2.0, kState = 0.5, kScan = 4.0;
+    const auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
+    double best = waves(rows * a.B) * (chunks + kStart);
+    for (int m = 2; m <= 32 && m <= chunks / 4; ++m) {
+      const int64_t len = (chunks + m - 1) / m, used = (chunks + len - 1) / len;
+      const double cost = waves(rows * a.B * used) * (len + kStart) + waves(rows * a.B * (used - 1)) * (kState * len + kStart) + kScan;
+      if (cost < 0.95 * best) {
+        best = cost;
+        cut.piece = static_cast<int>(len * kC);
+        cut.pieces = static_cast<int>(used);
+      }
+    }
+    cut.slots = static_cast<int64_t>(a.B) * cut.pieces;
+  }
+  if (!cut.slots || a.B + cut.slots > 65535) return Cut();
+  const int64_t page = static_cast<int64_t>(a.Hv) * a.dk * a.dv;
+  cut.state_bytes = cut.slots * page * 4;
+  cut.bytes = cut.state_bytes + cut.slots * a.Hv * 4;
+  return cut;
+}
+
 template <int DK, int BV, typename IO>
-int launch(const lin_prefill_args_t& a, cudaStream_t stream) {
+int launch(const lin_prefill_args_t& a, const Cut& cut, cudaStream_t stream) {
   constexpr bool bf = std::is_same<IO, __nv_bfloat16>::value;
   using L = Layout<DK, BV>;
-  static std::atomic<uint64_t> attr_done{0};
+  static std::atomic<uint64_t> full_done{0}, state_done{0};
   PrefillParams p;
   p.a = a;
   p.nvb = a.dv / BV;
+  p.piece = cut.piece;
+  p.pieces = cut.pieces;
+  p.slots = static_cast<int>(cut.slots);
+  p.slot_state = static_cast<float*>(a.workspace);
+  p.decay = reinterpret_cast<float*>(static_cast<char*>(a.workspace) + cut.state_bytes);
   const int B = a.cu_seqlens ? 1 : a.B;
   CUtensorMap mq, mk, mv, mo;
   int rc;
@@ -713,30 +924,26 @@ int launch(const lin_prefill_args_t& a, cudaStream_t stream) {
       (rc = io_map(&mv, bf, a.v, a.dv, a.Hv, a.T, B, a.v_sh, a.v_st, a.v_sb)) ||
       (rc = io_map(&mo, bf, a.o, a.dv, a.Hv, a.T, B, a.o_sh, a.o_st, a.o_sb)))
     return rc;
-  auto kern = lin_prefill_kernel<DK, BV, IO>;
-  if ((rc = ensure_smem_attr(kern, L::kBytes, attr_done))) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.Hv * p.nvb), static_cast<unsigned>(a.B));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = L::kBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, p, mq, mk, mv, mo) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return GDN_ERR_LAUNCH;
+  const unsigned rows = static_cast<unsigned>(a.Hv * p.nvb), slots = static_cast<unsigned>(cut.slots);
+  if (slots) {
+    const int64_t page = static_cast<int64_t>(a.Hv) * a.dk * a.dv;
+    if ((rc = ensure_smem_attr(lin_prefill_kernel<DK, BV, IO, false>, L::kBytes, state_done)) ||
+        (rc = launch_pdl(lin_prefill_kernel<DK, BV, IO, false>, dim3(rows, slots), kThreads, L::kBytes, stream, p, mq, mk, mv, mo)) ||
+        (rc = launch_pdl(lin_scan_kernel, dim3(static_cast<unsigned>((page + 1023) / 1024), static_cast<unsigned>(a.B)), 256, 0,
+                         stream, p)))
+      return rc;
   }
-  return GDN_OK;
+  if ((rc = ensure_smem_attr(lin_prefill_kernel<DK, BV, IO, true>, L::kBytes, full_done))) return rc;
+  // every sequence of a cut dense batch is cut: only slots then
+  const unsigned items = slots + (slots && !a.cu_seqlens ? 0u : static_cast<unsigned>(a.B));
+  return launch_pdl(lin_prefill_kernel<DK, BV, IO, true>, dim3(rows, items), kThreads, L::kBytes, stream, p, mq, mk, mv, mo);
 }
 
 template <typename IO>
-int dispatch(const lin_prefill_args_t& a, cudaStream_t stream) {
-  const bool wide = a.dv % 128 == 0;
-  if (a.dk == 64) return wide ? launch<64, 128, IO>(a, stream) : launch<64, 64, IO>(a, stream);
-  return wide ? launch<128, 128, IO>(a, stream) : launch<128, 64, IO>(a, stream);
+int dispatch(const lin_prefill_args_t& a, const Cut& cut, cudaStream_t stream) {
+  const bool wide = block_cols(a) == 128;
+  if (a.dk == 64) return wide ? launch<64, 128, IO>(a, cut, stream) : launch<64, 64, IO>(a, cut, stream);
+  return wide ? launch<128, 128, IO>(a, cut, stream) : launch<128, 64, IO>(a, cut, stream);
 }
 
 int validate(const lin_prefill_args_t* a) {
@@ -778,13 +985,23 @@ int validate(const lin_prefill_args_t* a) {
 }  // namespace
 }  // namespace gdn
 
-extern "C" size_t lin_prefill_workspace_size(const lin_prefill_args_t*) { return 0; }
+extern "C" size_t lin_prefill_workspace_size(const lin_prefill_args_t* a) {
+  if (gdn::validate(a)) return 0;
+  gdn::DeviceInfo di;
+  if (gdn::device_info(&di)) return 0;
+  return static_cast<size_t>(gdn::choose_cut(*a, di.sm_count).bytes);
+}
 
 extern "C" int lin_prefill_launch(const lin_prefill_args_t* a, gdn_stream_t stream) {
   int rc = gdn::validate(a);
   if (rc) return rc;
   gdn::DeviceInfo di;
   if ((rc = gdn::device_info(&di))) return rc;
+  const gdn::Cut cut = gdn::choose_cut(*a, di.sm_count);
+  if (cut.bytes) {
+    if (!a->workspace || a->workspace_bytes < static_cast<size_t>(cut.bytes)) return GDN_ERR_WORKSPACE;
+    if (!gdn::aligned16(a->workspace)) return GDN_ERR_ALIGN;
+  }
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return a->io_dtype == GDN_DT_BF16 ? gdn::dispatch<__nv_bfloat16>(*a, st) : gdn::dispatch<__half>(*a, st);
+  return a->io_dtype == GDN_DT_BF16 ? gdn::dispatch<__nv_bfloat16>(*a, cut, st) : gdn::dispatch<__half>(*a, cut, st);
 }

@@ -317,6 +317,56 @@ def test_prefill_long_few_heads_equals_pieces(pkg):
     check_prefill(torch.cat([o1, o2], 1)[0].cpu(), S2[0].cpu(), ref, io, k[0, -2000:], v[0])
 
 
+@pytest.mark.parametrize("T", [2048, 4097, 6000])
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+def test_prefill_long_in_place(pkg, T, io):
+    """Long enough for the time axis to be cut; the state is updated in place."""
+    B, Hqk, Hv, dk, dv = 2, 1, 2, 64, 64
+    q, k, v, g = make((B, T), Hqk, Hv, dk, dv, io, T, gmin=-0.05)
+    S0 = torch.randn(B, Hv, dk, dv, generator=torch.Generator().manual_seed(T))
+    st = S0.to(DEV)
+    o, fin = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st, scale=0.1, final_state=st, check=True)
+    for b in range(B):
+        ref = steps(q[b], k[b], v[b], g[b], S0[b], 0.1)
+        check_prefill(o[b].cpu(), fin[b].cpu(), ref, io, k[b], v[b])
+
+
+def test_prefill_packed_long_and_short(pkg):
+    """Packed sequences of which some are cut: one much longer than the rest, one of none, pages."""
+    Hqk, Hv, dk, dv, io = 1, 2, 64, 128, torch.bfloat16
+    lens = [100, 5000, 0, 2048, 2049, 3, 300]
+    T = sum(lens)
+    q, k, v, g = make((1, T), Hqk, Hv, dk, dv, io, 31, gmin=-0.05)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    pool = torch.randn(9, Hv, dk, dv, generator=torch.Generator().manual_seed(32))
+    index = torch.tensor([8, 1, 3, 0, -1, 5, 2], dtype=torch.int32)
+    st = pool.to(DEV)
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st, scale=0.1, index=index.to(DEV),
+                           cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV), check=True)
+    o, fin = o.cpu(), st.cpu()
+    for n, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        p = int(index[n])
+        if a == b:
+            assert torch.equal(fin[p], pool[p])
+            continue
+        ref = steps(q[0, a:b], k[0, a:b], v[0, a:b], g[0, a:b], pool[p] if p >= 0 else torch.zeros(Hv, dk, dv), 0.1)
+        check_prefill(o[0, a:b], fin[p] if p >= 0 else ref[1], ref, io, k[0, a:b], v[0, a:b])
+    assert torch.equal(fin[[4, 6, 7]], pool[[4, 6, 7]])
+
+
+def test_prefill_packed_unsound_offsets_of_long_sequences(pkg):
+    """Overlapping long sequences around an unsound one: reported, nothing outside is written."""
+    H, d, io, T = 1, 64, torch.bfloat16, 9000
+    q, k, v, g = (x.to(DEV) for x in make((1, T), H, H, d, d, io, 33))
+    cu = torch.tensor([0, 9000, 10, 9000, 20, 9000], dtype=torch.int32, device=DEV)
+    fin = torch.full((5, H, d, d), 3.0, device=DEV)
+    with pytest.raises(pkg.GDNError, match="index"):
+        pkg.lin_prefill(q, k, v, g, final_state=fin, cu_seqlens=cu, check=True)
+    assert bool((fin[[1, 3]] == 3).all())
+
+
 def test_graph_capture_on_another_stream(pkg):
     """Prefill and decode captured together, replayed on new inputs."""
     B, T, H, d, io = 2, 200, 2, 128, torch.bfloat16
