@@ -49,8 +49,15 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kWaitTries = 1u << 18;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
-// within this range e^(G_i - G_j) is taken as the product of e^G_i and e^-G_j
+// the factors of e^(G_i - G_j) stay within 2^-kNear .. 2^kNear
 constexpr float kNear = 100.f;
+// How a chunk's decays are factored, by the range of G (in powers of two):
+//   kNearMid    G spans at most 2 kNear: e^(G_i - M) e^(M - G_j), M its middle
+//   kNearBlock  no gate grows, and each block of 32 tokens spans kNear at most:
+//               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
+//               first of the two is zero so is P)
+//   kFar        else, as across a reset: e^(G_i - G_j) by itself
+enum { kNearMid = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
@@ -75,7 +82,7 @@ struct Layout {
   static constexpr int kGate = kS + DK / 64 * kSBlock;
   static constexpr int kGateStage = 2 * kC * 4;            // G or e^-G, w
   static constexpr int kBars = kGate + 2 * kGateStage;
-  static constexpr int kBytes = kBars + 320;
+  static constexpr int kBytes = kBars + 384;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -88,10 +95,12 @@ struct Bars {
   uint64_t v_ready[2], v_free[2], ds_done, ds_free, s_ready;
   uint64_t o_free, o_staged, zeroed, drain;
   float gamma[2];
-  int near_one[2];  // the chunk's e^G and e^-G both stay well inside fp32
+  float shift[2];   // e^M (1 unless kNearMid)
+  float ref[2][4];  // R_b
+  int form[2];      // kNearMid, kNearBlock, kFar
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 320, "barriers");
+static_assert(sizeof(Bars) <= 384, "barriers");
 
 struct PrefillParams {
   lin_prefill_args_t a;
@@ -358,14 +367,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(ok = wait_both(&bar.gfull[st], ph, &bar.full[kTileQ][st], ph))) break;
       if (c && !(ok = wait(&bar.qs_done, (c - 1) & 1))) break;
       tc::fence_after_sync();
-      const bool near_one = bar.near_one[st];
-      const float Gi = G[row];  // e^-G when near one
-      const float f = a.scale * (near_one ? __frcp_rn(Gi) : ex2(Gi));
+      const int form = bar.form[st];
+      const float own = G[row];  // e^(M - G_i), e^(R - G_i) or G_i
+      const float Gi = form == kNearBlock ? bar.ref[st][warp] - __log2f(own) : own;  // (of the other two forms)
+      const float f = a.scale * (form == kNearMid ? __frcp_rn(own) : ex2(Gi));
       const uint32_t f_hi = tc::pack2<true>(f, f);
       const uint32_t f_lo = tc::pack2<true>(f - tc::unpack_lo<true>(f_hi), f - tc::unpack_lo<true>(f_hi));
-      // bf16 near one: SC and QS both take Q' = scale e^G Q.  Else SC takes Q as it
-      // is, since e^G could leave the type's range, and Q' (bf16) follows it.
-      const bool shared_q = BF16 && near_one;
+      // bf16 and kNearMid: SC and QS both take Q' = scale e^(G - M) Q, and S^T carries
+      // e^M.  Else SC takes Q as it is, since the factor could leave the type's
+      // range, and Q' (bf16) follows it.
+      const bool shared_q = BF16 && form == kNearMid;
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         if (pass && !(ok = wait(&bar.sc_done, c & 1))) break;
@@ -407,12 +418,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
-          if (!near_one) {
+          if (form == kFar) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
-          } else if (!BF16) {
+          } else if (!shared_q) {
+            const float r = form == kNearMid ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] *= f;
+            for (int e = 0; e < 32; ++e) d[e] *= r;
           }
           tc::tmem_wait_ld();
 #pragma unroll
@@ -592,14 +604,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           mbar_arrive(&bar.ds_free);
         }
       }
-      if (!FULL) continue;
-      if (has_rows) {  // S^T rounded to bf16, the QS product's operand
+      if (!FULL || c + 1 == chunks) continue;
+      if (!(ok = wait(&bar.gfull[(c + 1) & 1], ((c + 1) >> 1) & 1))) break;
+      const float m = bar.shift[(c + 1) & 1];
+      if (has_rows) {  // e^M S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
           tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7),
-                     tc::pack2<true>(S[8 * i], S[8 * i + 1]), tc::pack2<true>(S[8 * i + 2], S[8 * i + 3]),
-                     tc::pack2<true>(S[8 * i + 4], S[8 * i + 5]), tc::pack2<true>(S[8 * i + 6], S[8 * i + 7]));
+                     tc::pack2<true>(m * S[8 * i], m * S[8 * i + 1]), tc::pack2<true>(m * S[8 * i + 2], m * S[8 * i + 3]),
+                     tc::pack2<true>(m * S[8 * i + 4], m * S[8 * i + 5]), tc::pack2<true>(m * S[8 * i + 6], m * S[8 * i + 7]));
         }
       }
       tc::fence_proxy_async();
@@ -675,17 +689,34 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) before = 0.f;
       if (lane == 31) after = 0.f;
       if (c >= 2 && !(ok = wait(&bar.gempty[st], ((c >> 1) & 1) ^ 1))) break;
-      float far = 0.f, gv[4], wv[4];
+      float gv[4], wv[4], lo = before + fwd[0], hi = lo;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         gv[e] = before + fwd[e];
         wv[e] = c * kC + lane * 4 + e < seq.len ? ex2(after + bwd[e]) : 0.f;
-        far = fmaxf(far, fabsf(gv[e]));
+        lo = fminf(lo, gv[e]);
+        hi = fmaxf(hi, gv[e]);
       }
-      const bool near_one = __all_sync(0xffffffffu, far <= kNear);
-      if (near_one) {
+      int form = kNearMid;
+      float ref = 0.f;  // M, or R of this lane's block (8 lanes)
+      if (FULL) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) gv[e] = ex2(-gv[e]);
+        for (int off = 1; off < 8; off <<= 1) {
+          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+        }
+        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kNear && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) <= 0.f);
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 8));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 8));
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 16));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 16));
+        const float end_of_block = __shfl_sync(0xffffffffu, gv[3], lane | 7);
+        form = hi - lo <= 2.f * kNear && fabsf(hi + lo) <= 2.f * kNear ? kNearMid : near_block ? kNearBlock : kFar;
+        ref = form == kNearMid ? 0.5f * (lo + hi) : end_of_block;
+        if (form != kFar) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) gv[e] = ex2(ref - gv[e]);
+        }
       }
       *reinterpret_cast<float4*>(G + lane * 4) = make_float4(gv[0], gv[1], gv[2], gv[3]);
       // the weights of two tokens in two parts of the I/O type: (hi, hi), (lo, lo)
@@ -698,8 +729,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       *reinterpret_cast<uint4*>(G + kC + lane * 4) = make_uint4(wp[0], wp[1], wp[2], wp[3]);
       if (lane == 0) {
         bar.gamma[st] = ex2(end);
-        bar.near_one[st] = near_one;
+        bar.shift[st] = form == kNearMid ? ex2(ref) : 1.f;
+        bar.form[st] = form;
       }
+      if (FULL && (lane & 7) == 7) bar.ref[st][lane >> 3] = ref;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.gfull[st]);
     }

@@ -12,13 +12,35 @@ import torch
 
 from . import _lib
 from ._lib import GDNError
-from .api import _dt, _require_cuda, _same_device, check_device_status, status_word
+from .api import _dt, _status_words, check_device_status, status_word
 
 
-def _launch(fn, args, dev: torch.device, what: str) -> None:
+# the current stream's handle without a Stream object around it (1.2 us less per call)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda dev: torch.cuda.current_stream(dev).cuda_stream
+_LOG, _LINEAR = _lib.GATE_LOG, _lib.GATE_LINEAR
+
+
+def _on(first, *others) -> int:
+    """The CUDA device that all tensors (None = absent) are on."""
+    dev = first.get_device()
+    if dev < 0:
+        raise GDNError("tensors must be CUDA tensors (there is no CPU implementation)", 6)
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise GDNError(f"all tensors must be on cuda:{dev}, got {t.device}", 2)
+    return dev
+
+
+def _status(dev: int) -> int:
+    w = _status_words.get(dev)
+    return (status_word(dev) if w is None else w).data_ptr()
+
+
+def _launch(fn, args, dev: int, what: str) -> None:
     """Calls a launcher on the tensors' device and that device's current stream."""
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == dev.index:
+    stream = _raw_stream(dev)
+    if torch.cuda.current_device() == dev:
         rc = fn(ctypes.byref(args), stream)
     else:
         with torch.cuda.device(dev):
@@ -28,35 +50,37 @@ def _launch(fn, args, dev: torch.device, what: str) -> None:
 
 
 def _check_io(q, k, v, out) -> None:
-    if k.dtype != q.dtype or v.dtype != q.dtype or out.dtype != q.dtype:
+    dt = q.dtype
+    if k.dtype is not dt or v.dtype is not dt or out.dtype is not dt:
         raise GDNError("q, k, v and out must share one dtype (bf16 or f16)", 4)
     if out.shape != v.shape:
         raise GDNError(f"out must have the shape of v, {tuple(v.shape)}, got {tuple(out.shape)}", 2)
-    for name, t in (("q", q), ("k", k), ("v", v), ("out", out)):
-        if t.stride(-1) != 1:
+
+
+def _check_rows(**strides) -> None:
+    for name, s in strides.items():
+        if s[-1] != 1:
             raise GDNError(f"{name}: the innermost dimension must be contiguous", 3)
 
 
-def _check_states(name: str, t, page: tuple) -> int:
+def _check_states(name: str, t, Hv: int, dk: int, dv: int) -> int:
     """Elements between the pages of a pool [P, Hv, d_k, d_v]; raises on any other layout."""
-    if t.dtype != torch.float32 or t.dim() != 4 or tuple(t.shape[1:]) != page:
-        raise GDNError(f"{name} must be fp32 [P, Hv, d_k, d_v] with pages of {page}, got "
-                       f"{t.dtype} {tuple(t.shape)}", 2)
-    if t.stride()[1:] != (page[1] * page[2], page[2], 1):
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.float32 or len(shape) != 4 or shape[1:] != (Hv, dk, dv):
+        raise GDNError(f"{name} must be fp32 [P, Hv, d_k, d_v] with pages of {(Hv, dk, dv)}, got "
+                       f"{t.dtype} {tuple(shape)}", 2)
+    if stride[1:] != (dk * dv, dv, 1) and not t[:1].is_contiguous():
         raise GDNError(f"{name}: each page must be contiguous", 3)
-    n = page[0] * page[1] * page[2]
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), n)
+    return stride[0] if shape[0] > 1 else max(stride[0], Hv * dk * dv)
 
 
-def _check_index(index, rows: int, pools, name: str = "index") -> None:
+def _check_index(index, rows: int, pages: int) -> None:
     if index is None:
-        for pool in pools:
-            if pool is not None and pool.shape[0] != rows:
-                raise GDNError(f"without index the states must have one page per sequence ({rows}), "
-                               f"got {pool.shape[0]}", 2)
-        return
-    if index.dtype != torch.int32 or tuple(index.shape) != (rows,) or not index.is_contiguous():
-        raise GDNError(f"{name} must be a contiguous int32 [{rows}] tensor", 2)
+        if pages != rows:
+            raise GDNError(f"without index the states must have one page per sequence ({rows}), "
+                           f"got {pages}", 2)
+    elif index.dtype is not torch.int32 or index.shape != (rows,) or not index.is_contiguous():
+        raise GDNError(f"index must be a contiguous int32 [{rows}] tensor", 2)
 
 
 def lin_decode(q, k, v, g, state, *, scale: float = 1.0, out=None, gate: str = "log",
@@ -74,45 +98,50 @@ def lin_decode(q, k, v, g, state, *, scale: float = 1.0, out=None, gate: str = "
     holds, is treated as idle and reported (``check=True`` synchronises and
     raises).  Rows without a page leave ``state_out`` as it was.
     """
-    dev = _require_cuda(q, k, v, g, state)
+    dev = _on(q, k, v, g, state, state_out, out, index)
     if out is None:
-        out = torch.empty(v.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     if state_out is None:
         state_out = state
-    _same_device(q, out=out, state_out=state_out, index=index)
-    a = _decode_args(q, k, v, g, state, state_out, out, index, scale, gate)
-    a.status = status_word(dev).data_ptr()
+    a = _decode_args(q, k, v, g, state, state_out, out, index, scale, gate, _status(dev))
     _launch(_lib.load().lin_decode_launch, a, dev, "lin_decode")
     if check:
         check_device_status(dev)
     return out
 
 
-def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate) -> _lib.LinDecodeArgs:
-    if q.dim() != 3 or k.shape != q.shape or v.dim() != 3 or v.shape[0] != q.shape[0]:
+def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate,
+                 status=None) -> _lib.LinDecodeArgs:
+    shape, v_shape = q.shape, v.shape
+    if len(shape) != 3 or k.shape != shape or len(v_shape) != 3 or v_shape[0] != shape[0]:
         raise GDNError("q, k must be [B, Hqk, d_k] and v [B, Hv, d_v]", 2)
-    B, Hqk, dk = q.shape
-    _, Hv, dv = v.shape
+    B, Hqk, dk = shape
+    _, Hv, dv = v_shape
     _check_io(q, k, v, out)
-    g_sb = 0
-    if g.dim() == 2:
-        g_sb = g.stride(0)
-    if tuple(g.shape) not in ((B, Hv), (Hv,)):
+    qs, ks, vs, os, gs = q.stride(), k.stride(), v.stride(), out.stride(), g.stride()
+    if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os[2] != 1:
+        _check_rows(q=qs, k=ks, v=vs, out=os)
+    if g.shape == (B, Hv):
+        g_sb, g_sh = gs
+    elif g.shape == (Hv,):
+        g_sb, g_sh = 0, gs[0]
+    else:
         raise GDNError(f"g must be [B, Hv] = {(B, Hv)} or [Hv], got {tuple(g.shape)}", 2)
     if gate not in ("log", "linear"):
         raise GDNError("gate must be 'log' (decay = exp(g)) or 'linear' (decay = g)", 4)
-    page = (Hv, dk, dv)
-    in_sp, out_sp = _check_states("state", state, page), _check_states("state_out", state_out, page)
-    if state_out.shape[0] != state.shape[0]:
-        raise GDNError("state_out must have as many pages as state", 2)
-    _check_index(index, B, (state,))
+    in_sp = out_sp = _check_states("state", state, Hv, dk, dv)
+    pages = state.shape[0]
+    if state_out is not state:
+        out_sp = _check_states("state_out", state_out, Hv, dk, dv)
+        if state_out.shape[0] != pages:
+            raise GDNError("state_out must have as many pages as state", 2)
+    _check_index(index, B, pages)
     return _lib.LinDecodeArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(),
-        state_out.data_ptr(), out.data_ptr(), index.data_ptr() if index is not None else None,
-        q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-        out.stride(0), out.stride(1), g_sb, g.stride(-1), in_sp, out_sp,
-        B, Hqk, Hv, dk, dv, state.shape[0], _dt(q, "q"), _dt(g, "g"),
-        _lib.GATE_LOG if gate == "log" else _lib.GATE_LINEAR, scale, None)
+        state_out.data_ptr(), out.data_ptr(), None if index is None else index.data_ptr(),
+        qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], g_sb, g_sh, in_sp, out_sp,
+        B, Hqk, Hv, dk, dv, pages, _dt(q, "q"), _dt(g, "g"), _LOG if gate == "log" else _LINEAR,
+        scale, status)
 
 
 def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlens=None,
@@ -138,9 +167,9 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
     (``check=True``).  q, k, v and out may be strided views whose rows are
     contiguous and 16-byte aligned.
     """
-    dev = _require_cuda(q, k, v, g)
+    dev = _on(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, workspace)
     if out is None:
-        out = torch.empty(v.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     if final_state is None:
         if index is not None:
             if initial_state is None:
@@ -149,20 +178,18 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
         elif v.dim() == 4 and q.dim() == 4:
             rows = v.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
             final_state = torch.empty((rows, v.shape[2], q.shape[3], v.shape[3]),
-                                      dtype=torch.float32, device=dev)
-    _same_device(q, initial_state=initial_state, final_state=final_state, out=out,
-                 cu_seqlens=cu_seqlens, index=index)
-    a = _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale)
-    a.status = status_word(dev).data_ptr()
+                                      dtype=torch.float32, device=q.device)
+    a = _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale,
+                      _status(dev))
     L = _lib.load()
     need = L.lin_prefill_workspace_size(ctypes.byref(a))
     if need:
         # from the allocator on the current stream, so that calls on other streams
         # and captured graphs have workspaces of their own
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-        elif workspace.device != dev or not workspace.is_contiguous():
-            raise GDNError(f"workspace must be a contiguous tensor on {dev}", 2)
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        elif not workspace.is_contiguous():
+            raise GDNError("workspace must be a contiguous tensor", 2)
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _launch(L.lin_prefill_launch, a, dev, "lin_prefill")
     if check:
@@ -170,39 +197,40 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
     return out, final_state
 
 
-def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index,
-                  scale) -> _lib.LinPrefillArgs:
-    if q.dim() != 4 or k.shape != q.shape or v.dim() != 4 or v.shape[:2] != q.shape[:2]:
+def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale,
+                  status=None) -> _lib.LinPrefillArgs:
+    shape, v_shape = q.shape, v.shape
+    if len(shape) != 4 or k.shape != shape or len(v_shape) != 4 or v_shape[:2] != shape[:2]:
         raise GDNError("q, k must be [B, T, Hqk, d_k] and v [B, T, Hv, d_v]", 2)
-    B, T, Hqk, dk = q.shape
-    Hv, dv = v.shape[2:]
+    B, T, Hqk, dk = shape
+    _, _, Hv, dv = v_shape
     _check_io(q, k, v, out)
-    if tuple(g.shape) == (B, T, Hv):
-        g_s = g.stride()
-    elif tuple(g.shape) == (Hv,):
-        g_s = (0, 0, g.stride(0))
-    else:
+    qs, ks, vs, os, gs = q.stride(), k.stride(), v.stride(), out.stride(), g.stride()
+    if qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or os[3] != 1:
+        _check_rows(q=qs, k=ks, v=vs, out=os)
+    if g.shape == (Hv,):
+        gs = (0, 0, gs[0])
+    elif g.shape != (B, T, Hv):
         raise GDNError(f"g must be [B, T, Hv] = {(B, T, Hv)} or [Hv], got {tuple(g.shape)}", 2)
     seqs = B
     if cu_seqlens is not None:
-        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 \
+        if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2 \
                 or not cu_seqlens.is_contiguous():
             raise GDNError("cu_seqlens must be a contiguous int32 [N + 1] tensor", 2)
         if B != 1:
             raise GDNError("packed sequences (cu_seqlens) need a batch of one", 2)
         seqs = cu_seqlens.numel() - 1
-    page = (Hv, dk, dv)
-    fin_sp, in_sp = _check_states("final_state", final_state, page), 0
+    fin_sp, in_sp = _check_states("final_state", final_state, Hv, dk, dv), 0
+    pages = final_state.shape[0]
     if initial_state is not None:
-        in_sp = _check_states("initial_state", initial_state, page)
-        if initial_state.shape[0] != final_state.shape[0]:
+        in_sp = _check_states("initial_state", initial_state, Hv, dk, dv)
+        if initial_state.shape[0] != pages:
             raise GDNError("initial_state and final_state must have as many pages", 2)
-    _check_index(index, seqs, (initial_state, final_state))
+    _check_index(index, seqs, pages)
     return _lib.LinPrefillArgs(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
-        initial_state.data_ptr() if initial_state is not None else None, final_state.data_ptr(),
-        out.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None,
-        index.data_ptr() if index is not None else None,
-        *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *out.stride()[:3], *g_s, in_sp, fin_sp,
-        seqs, T, Hqk, Hv, dk, dv, final_state.shape[0], _dt(q, "q"), _dt(g, "g"), scale,
-        None, 0, None)
+        None if initial_state is None else initial_state.data_ptr(), final_state.data_ptr(),
+        out.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+        None if index is None else index.data_ptr(),
+        *qs[:3], *ks[:3], *vs[:3], *os[:3], *gs, in_sp, fin_sp,
+        seqs, T, Hqk, Hv, dk, dv, pages, _dt(q, "q"), _dt(g, "g"), scale, None, 0, status)

@@ -20,42 +20,47 @@ import torch
 
 from . import _lib
 from ._lib import GDNError
-from .api import _require_cuda, _same_device, check_device_status, status_word
-from .lin import _launch
+from .api import check_device_status
+from .lin import _launch, _on, _status
 
 
-def _pools(pools) -> tuple[list, "ctypes.Array | None"]:
+def _pools(pools) -> tuple[list, "ctypes.Array"]:
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     if len(pools) > _lib.PAGES_MAX_POOLS:
         raise GDNError(f"at most {_lib.PAGES_MAX_POOLS} pools in a call, got {len(pools)}", 2)
-    arr = (_lib.PagesPool * max(1, len(pools)))()
-    for i, p in enumerate(pools):
+    flat = []
+    for p in pools:
         if p.dim() < 2 or p.shape[0] != pools[0].shape[0]:
             raise GDNError("pools must be [P, ...] tensors with the same number of pages", 2)
-        if not p[0].is_contiguous():
+        P, size = p.shape[0], p.element_size()
+        n = p.numel() // P * size if P else 0
+        if not p.is_contiguous() and not p[:1].is_contiguous():
             raise GDNError("each page of a pool must be contiguous", 3)
-        size, n = p.element_size(), p[0].numel()
-        arr[i] = (p.data_ptr(), (p.stride(0) if p.shape[0] > 1 else n) * size, n * size)
-    return pools, arr
+        flat.append((p.data_ptr(), p.stride(0) * size if P > 1 else n, n))
+    return pools, (_lib.PagesPool * max(1, len(flat)))(*flat)
 
 
 def _int32(name: str, t, shape=None) -> None:
-    if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() \
-            or (shape is not None and tuple(t.shape) != shape):
+    if t.dtype is not torch.int32 or t.dim() != 1 or not t.is_contiguous() \
+            or (shape is not None and t.shape != shape):
         raise GDNError(f"{name} must be a contiguous int32 [{shape[0] if shape else 'n'}] tensor", 2)
 
 
-def _call(fn: str, dev, pages, *, pools=(), arr=None, used=None, used_out=None, n=0, src=None,
-          dst=None, remap=None, count=None, check=False) -> None:
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(fn: str, like, dev: int, pages: int, *, pools=(), arr=None, used=None, used_out=None, n=0,
+          src=None, dst=None, remap=None, count=None, check=False) -> None:
     if not 1 <= pages <= _lib.PAGES_MAX_PAGES:
         raise GDNError(f"a pool must have 1 to {_lib.PAGES_MAX_PAGES} pages, got {pages}", 2)
-    ptr = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
-    a = _lib.PagesArgs(arr, len(pools), pages, ptr(used), ptr(used_out), n, ptr(src), ptr(dst),
-                       ptr(remap), ptr(count), None, 0, status_word(dev).data_ptr())
+    a = _lib.PagesArgs(arr, len(pools), pages, _ptr(used), _ptr(used_out), n, _ptr(src), _ptr(dst),
+                       _ptr(remap), _ptr(count), None, 0, _status(dev))
     L = _lib.load()
-    # from the allocator on the current stream: no two calls in flight share it
-    ws = torch.empty(max(16, L.pages_workspace_size(ctypes.byref(a))), dtype=torch.uint8, device=dev)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    need = L.pages_workspace_size(ctypes.byref(a)) if fn != "pages_free_launch" else 0
+    if need:  # from the allocator on the current stream: no two calls in flight share it
+        ws = torch.empty(need, dtype=torch.uint8, device=like.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), need
     _launch(getattr(L, fn), a, dev, fn.removesuffix("_launch"))
     if check:
         check_device_status(dev)
@@ -71,10 +76,10 @@ def pages_copy(pools, src, dst, *, check: bool = False) -> None:
     pools, arr = _pools(pools)
     if not pools:
         raise GDNError("pages_copy needs a pool", 1)
-    dev = _require_cuda(*pools, src, dst)
+    dev = _on(src, dst, *pools)
     _int32("src", src)
     _int32("dst", dst, tuple(src.shape))
-    _call("pages_copy_launch", dev, pools[0].shape[0], pools=pools, arr=arr, n=src.numel(), src=src,
+    _call("pages_copy_launch", src, dev, pools[0].shape[0], pools=pools, arr=arr, n=src.numel(), src=src,
           dst=dst, check=check)
 
 
@@ -86,7 +91,7 @@ def pages_fork(pools, used, src, *, out=None, used_out=None, check: bool = False
     The result is -1 where src[i] is negative and, with a device error, where
     src[i] is out of range or free, or no free page is left."""
     pools, arr = _pools(pools)
-    dev = _require_cuda(*pools, used, src)
+    dev = _on(used, src, out, used_out, *pools)
     _int32("src", src)
     if pools and used.numel() != pools[0].shape[0]:
         raise GDNError(f"used must be [P] = [{pools[0].shape[0]}], got {tuple(used.shape)}", 2)
@@ -96,7 +101,7 @@ def pages_fork(pools, used, src, *, out=None, used_out=None, check: bool = False
 def pages_alloc(used, n: int, *, out=None, used_out=None, check: bool = False) -> torch.Tensor:
     """Takes the n lowest free pages: int32 [n], -1 (with a device error) once
     none is left.  Their contents are left as they are."""
-    dev = _require_cuda(used)
+    dev = _on(used, out, used_out)
     if n < 0:
         raise GDNError(f"n must not be negative, got {n}", 2)
     return _fork(dev, [], None, used, None, n, out, used_out, check)
@@ -105,12 +110,11 @@ def pages_alloc(used, n: int, *, out=None, used_out=None, check: bool = False) -
 def _fork(dev, pools, arr, used, src, n, out, used_out, check):
     used_out = used if used_out is None else used_out
     if out is None:
-        out = torch.empty(n, dtype=torch.int32, device=dev)
-    _same_device(used, out=out, used_out=used_out)
+        out = used.new_empty(n)
     _int32("used", used)
     _int32("used_out", used_out, tuple(used.shape))
     _int32("out", out, (n,))
-    _call("pages_fork_launch", dev, used.numel(), pools=pools, arr=arr, used=used, used_out=used_out,
+    _call("pages_fork_launch", used, dev, used.numel(), pools=pools, arr=arr, used=used, used_out=used_out,
           n=n, src=src, dst=out, check=check)
     return out
 
@@ -119,13 +123,12 @@ def pages_free(used, index, *, used_out=None, check: bool = False) -> torch.Tens
     """Marks the pages index[i] (int32 [n]) free in ``used`` (or ``used_out``,
     which is returned).  Negative entries are skipped; an entry out of range, or
     of a page that is free already, is a device error."""
-    dev = _require_cuda(used, index)
+    dev = _on(used, index, used_out)
     used_out = used if used_out is None else used_out
-    _same_device(used, used_out=used_out)
     _int32("used", used)
     _int32("used_out", used_out, tuple(used.shape))
     _int32("index", index)
-    _call("pages_free_launch", dev, used.numel(), used=used, used_out=used_out, n=index.numel(),
+    _call("pages_free_launch", used, dev, used.numel(), used=used, used_out=used_out, n=index.numel(),
           src=index, check=check)
     return used_out
 
@@ -140,24 +143,22 @@ def pages_compact(pools, used, *, index=None, index_out=None, used_out=None, che
     ``used`` is updated in place (or into ``used_out``).  Pages behind the first
     ``count`` keep their bytes."""
     pools, arr = _pools(pools)
-    dev = _require_cuda(used, *pools)
+    dev = _on(used, used_out, index, index_out, *pools)
     used_out = used if used_out is None else used_out
     P, n = used.numel(), 0
     if pools and P != pools[0].shape[0]:
         raise GDNError(f"used must be [P] = [{pools[0].shape[0]}], got {tuple(used.shape)}", 2)
     _int32("used", used)
     _int32("used_out", used_out, tuple(used.shape))
-    remap = torch.empty(P, dtype=torch.int32, device=dev)
-    count = torch.empty(1, dtype=torch.int32, device=dev)
+    remap, count = used.new_empty(P), used.new_empty(1)
     if index is not None:
         n = index.numel()
         _int32("index", index)
         if index_out is None:
-            index_out = torch.empty(n, dtype=torch.int32, device=dev)
+            index_out = used.new_empty(n)
         _int32("index_out", index_out, (n,))
     elif index_out is not None:
         raise GDNError("index_out needs index", 1)
-    _same_device(used, used_out=used_out, index=index, index_out=index_out)
-    _call("pages_compact_launch", dev, P, pools=pools, arr=arr, used=used, used_out=used_out, n=n,
+    _call("pages_compact_launch", used, dev, P, pools=pools, arr=arr, used=used, used_out=used_out, n=n,
           src=index, dst=index_out, remap=remap, count=count, check=check)
     return remap, count, index_out

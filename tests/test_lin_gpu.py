@@ -191,6 +191,27 @@ def test_prefill_gates(pkg, gate, g_dtype, gmin):
     check_prefill(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], gg, S0[0], 1.0), io, k[0], v[0])
 
 
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gmin,gmax", [(-1.0, 0.0), (-2.0, 0.0), (-2.5, 0.0), (-3.5, 0.0), (-0.4, 0.4), (0.0, 0.05)])
+def test_prefill_gate_ranges(pkg, io, gmin, gmax):
+    """Decays over a chunk from mild to beyond fp32's range, and gates that grow."""
+    T, d = 300, 64
+    q, k, v, _ = make((1, T), 1, 2, d, d, io, 18)
+    g = gmin + (gmax - gmin) * torch.rand(1, T, 2, generator=torch.Generator().manual_seed(19))
+    g[0, :, 1] = g[0, :, 1].sort().values  # and a head whose decay changes along the way
+    S0 = torch.randn(1, 2, d, d)
+    v = (v.float() * 2.0 ** -4).to(io)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=0.125, check=True)
+    ro, rS, oa, Sa = steps(q[0], k[0], v[0], g[0], S0[0], 0.125)
+    heads = [0, 1]
+    if io == torch.float16 and gmax == 0.4:
+        # the second head's exact outputs reach 2.3e13: no f16 holds them
+        assert float(ro[:, 1].abs().max()) > torch.finfo(io).max
+        heads = [0]
+    check_prefill(o[0, :, heads].cpu(), S[0, heads].cpu(), (ro[:, heads], rS[heads], oa[:, heads], Sa[heads]), io,
+                  k[0], v[0])
+
+
 @pytest.mark.parametrize("g_reset", [float("-inf"), -200.0, -1e30])
 def test_prefill_resets(pkg, g_reset):
     """A decay of zero at some tokens starts the sequence anew there, also inside a chunk."""
