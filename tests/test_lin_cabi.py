@@ -103,8 +103,9 @@ def test_prefill_refuses(pkg, over, code):
 def pages_args(pkg, pool=None, **over):
     L = pkg._lib
     pools = (L.PagesPool * 1)(pool or (BASE, 4096, 4096))
-    a = L.PagesArgs(pools, 1, 8, BASE, BASE, 4, BASE + 4096, BASE + 8192, BASE + 12288, BASE + 16384,
-                    BASE + 20480, 4096, None)
+    M = 1 << 24
+    a = L.PagesArgs(pools, 1, 8, BASE, BASE, 4, BASE + M, BASE + 2 * M, BASE + 3 * M, BASE + 4 * M,
+                    BASE + 5 * M, 4096, None)
     for k, v in over.items():
         setattr(a, k, v)
     a._keep = pools
@@ -116,11 +117,34 @@ def pages_args(pkg, pool=None, **over):
     ({"pages": 0}, 2), ({"pages": (1 << 19) + 1}, 2), ({"n": -1}, 2), ({"n_pools": 65}, 2),
     ({"pool": (0, 4096, 4096)}, 1), ({"pool": (BASE, 4080, 4096)}, 2), ({"pool": (BASE, 4096, 4088)}, 3),
     ({"pool": (BASE, 4100, 4096)}, 3), ({"pool": (BASE + 8, 4096, 4096)}, 3),
-    ({"dst": 0}, 1), ({"workspace": 0}, 7), ({"workspace_bytes": 12}, 7), ({"workspace": BASE + 2}, 3),
+    ({"dst": 0}, 1),
+    # (small calls need no workspace)
+    ({"pages": 5000, "n": 3000, "workspace": 0}, 7), ({"pages": 5000, "n": 3000, "workspace_bytes": 12}, 7),
+    ({"pages": 5000, "n": 3000, "workspace": BASE + 2, "workspace_bytes": 1 << 20}, 3),
 ])
 def test_pages_refuse(pkg, fn, over, code):
     a = pages_args(pkg, **over)
     assert getattr(pkg._lib.load(), f"pages_{fn}_launch")(ctypes.byref(a), None) == code
+
+
+@pytest.mark.parametrize("fn,over", [
+    ("fork", {"dst": BASE + (1 << 24) + 4}),       # entries and results share memory
+    ("fork", {"used_out": BASE + 16}),             # flags shifted against themselves
+    ("fork", {"dst": BASE + 16}), ("fork", {"src": BASE}),
+    ("free", {"src": BASE + 8}),
+    ("compact", {"dst": BASE + (1 << 24) + 4}), ("compact", {"remap": BASE}), ("compact", {"count": BASE + 3 * (1 << 24)}),
+    ("compact", {"src": BASE + 8}),
+])
+def test_pages_refuse_shared_memory(pkg, fn, over):
+    a = pages_args(pkg, **over)
+    assert getattr(pkg._lib.load(), f"pages_{fn}_launch")(ctypes.byref(a), None) == 2
+
+
+def test_pages_workspace(pkg):
+    L = pkg._lib.load()
+    assert L.pages_workspace_size(ctypes.byref(pages_args(pkg, pages=2048, n=2048))) == 0
+    assert L.pages_workspace_size(ctypes.byref(pages_args(pkg, pages=2049, n=4))) == 4 * 2049
+    assert L.pages_workspace_size(ctypes.byref(pages_args(pkg, pages=8, n=3000, remap=0))) == 4 * 3000
 
 
 def test_pages_refuse_missing_flags(pkg):

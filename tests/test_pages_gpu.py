@@ -31,7 +31,7 @@ def same(pools, want):
     return all(torch.equal(a, b) for a, b in zip(pools, want))
 
 
-@pytest.mark.parametrize("P,n", [(2, 1), (40, 17), (1500, 700)])
+@pytest.mark.parametrize("P,n", [(2, 1), (40, 17), (1500, 700), (2049, 5), (5000, 2300)])
 def test_copy(pkg, P, n):
     pools = make_pools(P, P)
     want = copies(pools)
