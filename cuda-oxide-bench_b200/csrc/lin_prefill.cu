@@ -16,10 +16,10 @@
 //
 // Warps (19): R 0-3 (a row of the chunk per thread), V 4-7, S 8-15, TMA 16,
 // gates 17, MMA 18.  Per chunk, in the MMA warp's order:
-//   SC  scores = Q' K^T            Q' = scale e^G Q in TMEM (R); R turns them into
+//   SC  scores = Q K^T             Q in TMEM (R); R turns them into
 //                                  P, packed over the scores' own columns
 //   D0  dS^T  = V''^T K            of the chunk's first 64 tokens, V'' in TMEM (V)
-//   QS  O     = Q' S               S^T in shared memory
+//   QS  O     = Q S                S^T in shared memory
 //   D1  dS^T += V''^T K            of the others; then S reads dS and rewrites S^T
 //   PV  O    += P V                then S writes O out
 // All five take A from TMEM: a product with both operands in shared memory
@@ -53,7 +53,7 @@ constexpr float kLowest = -160.f;
 constexpr float kNear = 100.f;
 // How a chunk's decays are factored, by the range of G (in powers of two):
 //   kNearMid    G spans at most 2 kNear: e^(G_i - M) e^(M - G_j), M its middle
-//   kNearBlock  no gate grows, and each block of 32 tokens spans kNear at most:
+//   kNearBlock  no gate grows, and each block of 32 tokens spans at most kNear:
 //               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
@@ -68,19 +68,16 @@ constexpr uint32_t kTmDS = 384;   // dS^T fp32 [DK]
 
 template <int DK, int BV>
 struct Layout {
-  static constexpr int kQ = 0;
-  static constexpr int kK = kQ + DK / 64 * kTile;
+  // K and V in two stages; Q, which R takes into TMEM at once, in one
+  static constexpr int kK = 0;
   static constexpr int kV = kK + DK / 64 * kTile;
   static constexpr int kStage = kV + BV / 64 * kTile;
-  static constexpr int kStages = 2;
-  static constexpr int kS = kStages * kStage;              // S^T bf16 [BV][DK], 64-wide blocks
+  static constexpr int kQ = 2 * kStage;
+  static constexpr int kS = kQ + DK / 64 * kTile;          // e^M S^T bf16 [BV][DK], 64-wide blocks
   static constexpr int kSBlock = BV * 128;
-  // O of a chunk is staged in its K tile (read last by D1), or in its V tile (read
-  // last by PV, and wanted again a little sooner) where the K tile is too small
-  static constexpr bool kOInK = DK >= BV;
-  static constexpr int kO = kOInK ? kK : kV;
-  static constexpr int kGate = kS + DK / 64 * kSBlock;
-  static constexpr int kGateStage = 2 * kC * 4;            // G or e^-G, w
+  static constexpr int kO = kS + DK / 64 * kSBlock;
+  static constexpr int kGate = kO + BV / 64 * kTile;
+  static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
   static constexpr int kBars = kGate + 2 * kGateStage;
   static constexpr int kBytes = kBars + 384;
   static_assert(kBytes <= 232448, "shared memory");
@@ -89,11 +86,11 @@ struct Layout {
 enum { kTileQ = 0, kTileK = 1, kTileV = 2 };
 
 struct Bars {
-  uint64_t full[3][2], empty[3][2];  // of the Q, K, V tiles
+  uint64_t full[3][2], empty[3][2];  // of the Q (one stage), K, V tiles
   uint64_t gfull[2], gempty[2];
   uint64_t sc_done, q_ready, q2_ready, qs_done, p_ready, pv_done;
   uint64_t v_ready[2], v_free[2], ds_done, ds_free, s_ready;
-  uint64_t o_free, o_staged, zeroed, drain;
+  uint64_t o_free, o_staged, o_stored, zeroed, drain;
   float gamma[2];
   float shift[2];   // e^M (1 unless kNearMid)
   float ref[2][4];  // R_b
@@ -343,6 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.s_ready, 8);
     mbar_init(&bar.o_free, 4);
     mbar_init(&bar.o_staged, 4);
+    mbar_init(&bar.o_stored, 1);
     mbar_init(&bar.zeroed, 4);
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
@@ -361,52 +359,54 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
     for (int c = 0; c < chunks; ++c) {
       const int st = c & 1;
-      const uint32_t ph = (c >> 1) & 1;
       const float* G = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage);
       // Q into the columns that the last chunk's QS has read
-      if (!(ok = wait_both(&bar.gfull[st], ph, &bar.full[kTileQ][st], ph))) break;
+      if (!(ok = wait_both(&bar.gfull[st], (c >> 1) & 1, &bar.full[kTileQ][0], c & 1))) break;
       if (c && !(ok = wait(&bar.qs_done, (c - 1) & 1))) break;
       tc::fence_after_sync();
       const int form = bar.form[st];
       const float own = G[row];  // e^(M - G_i), e^(R - G_i) or G_i
       const float Gi = form == kNearBlock ? bar.ref[st][warp] - __log2f(own) : own;  // (of the other two forms)
       const float f = a.scale * (form == kNearMid ? __frcp_rn(own) : ex2(Gi));
-      const uint32_t f_hi = tc::pack2<true>(f, f);
-      const uint32_t f_lo = tc::pack2<true>(f - tc::unpack_lo<true>(f_hi), f - tc::unpack_lo<true>(f_hi));
-      // bf16 and kNearMid: SC and QS both take Q' = scale e^(G - M) Q, and S^T carries
-      // e^M.  Else SC takes Q as it is, since the factor could leave the type's
-      // range, and Q' (bf16) follows it.
-      const bool shared_q = BF16 && form == kNearMid;
+      // SC takes Q as it is.  bf16, and not kFar: so does QS; O then lacks the row's
+      // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: of rows
+      // whose factor is below 2^-kNear, QS takes zeros, and P carries it.)  Else P
+      // carries the row's factor, which its type could not do without, and QS takes
+      // Q' = scale e^G Q (bf16) written over Q.
+      const bool by_block = BF16 && form == kNearBlock, live = Gi >= -kNear;
+      const bool plain_q = BF16 && (form == kNearMid || (by_block && __all_sync(0xffffffffu, live)));
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         if (pass && !(ok = wait(&bar.sc_done, c & 1))) break;
         tc::fence_after_sync();
-        if (!pass || !shared_q) {
+        if (!pass || !plain_q) {
 #pragma unroll 1
           for (int b = 0; b < DK / 64; ++b) {
             uint32_t u[2][16];
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-              lds128(smem + st * L::kStage + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
-            if (pass || shared_q) {
+              lds128(smem + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
+            if (pass) {
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 uint32_t& w = u[i >> 4][i & 15];
-                w = BF16 ? tc::fma2<true>(w, f_hi, tc::mul2<true>(w, f_lo))
-                         : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
+                w = by_block ? (live ? w : 0u)
+                             : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
               }
             }
-            tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
+          tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
             tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
           }
           tc::tmem_wait_st();
           tc::fence_before_sync();
           __syncwarp();
         }
-        if (lane == 0) mbar_arrive(pass ? &bar.q2_ready : &bar.q_ready);
+        if (lane == 0) {
+          mbar_arrive(pass ? &bar.q2_ready : &bar.q_ready);
+          if (pass != plain_q) mbar_arrive(&bar.empty[kTileQ][0]);  // read for the last time
+        }
       }
       if (!ok) break;
-      if (lane == 0) mbar_arrive(&bar.empty[kTileQ][st]);
       // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
 #pragma unroll 1
       for (int b = 0; b < 4; ++b) {
@@ -421,7 +421,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (form == kFar) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
-          } else if (!shared_q) {
+          } else if (by_block) {
+            // the block's factor in two steps of at most 2^kNear, or the row's as well
+            const float R = bar.ref[st][b];
+            const float r0 = live ? ex2(-0.5f * R) : a.scale * ex2(Gi - R), r1 = live ? r0 : 1.f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) d[e] = d[e] * r0 * r1;
+          } else if (!BF16) {
             const float r = form == kNearMid ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] *= r;
@@ -491,11 +497,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.v_ready[half]);
     };
-    // O of chunk c: a token per thread, packed into shared memory
+    // O of chunk c: a token per thread, times the row's factor, packed into shared memory
+    float factor = 1.f;
     const auto output = [&](int c) {
-      const int st = c & 1;
-      unsigned char* o = smem + st * L::kStage + L::kO;
-      if (!wait(&bar.pv_done, c & 1)) return false;
+      unsigned char* o = smem + L::kO;
+      if (!wait(&bar.pv_done, c & 1) || (c && !wait(&bar.o_stored, (c - 1) & 1))) return false;
       tc::fence_after_sync();
 #pragma unroll 1
       for (int b = 0; b < BV / 32; ++b) {
@@ -507,8 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float* y = &x[e >> 1][(e & 1) * 8];
-          tc::sts128(to + tc::sw128_offset(row, (b & 1) * 4 + e), tc::pack2<BF16>(y[0], y[1]), tc::pack2<BF16>(y[2], y[3]),
-                     tc::pack2<BF16>(y[4], y[5]), tc::pack2<BF16>(y[6], y[7]));
+          tc::sts128(to + tc::sw128_offset(row, (b & 1) * 4 + e), tc::pack2<BF16>(factor * y[0], factor * y[1]),
+                     tc::pack2<BF16>(factor * y[2], factor * y[3]), tc::pack2<BF16>(factor * y[4], factor * y[5]),
+                     tc::pack2<BF16>(factor * y[6], factor * y[7]));
         }
       }
       tc::fence_before_sync();
@@ -562,7 +569,20 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (before >= 0 && !(ok = wait(&bar.v_free[before & 1], (before >> 1) & 1))) break;
         tc::fence_after_sync();
         parts(c, half);
-        if (half && lane == 0) mbar_arrive(&bar.gempty[st]);
+        if (half) {
+          if (FULL) {
+            const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];
+            const int form = bar.form[st];
+            factor = 1.f;
+            if (BF16 && form == kNearMid) factor = a.scale * __frcp_rn(own);
+            if (BF16 && form == kNearBlock) {
+              const float Gi = bar.ref[st][quarter] - __log2f(own);
+              if (Gi >= -kNear) factor = a.scale * ex2(Gi);
+            }
+            __syncwarp();
+          }
+          if (lane == 0) mbar_arrive(&bar.gempty[st]);
+        }
       }
       if (FULL && c && !half && !(ok = output(c - 1))) break;
     }
@@ -627,29 +647,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kWarpTma) {
     if (tc::elect_one()) {
-      // in the order in which the tiles come free; a tile's barrier is armed only
-      // then, when its last load is known to be complete
+      // In the order in which the tiles come free (the second chunk's Q waits for the
+      // first's); a tile's barrier is armed only then, its last load being complete.
       int armed[3] = {0, 0, 0};
       for (int c = 0; c < chunks && ok; ++c) {
-        const int st = c & 1;
-        unsigned char* stage = smem + st * L::kStage;
         const int t = seq.start + c * kC;
-        const auto load = [&](int tile, const CUtensorMap* map, int at, int blocks, int x, int head) {
-          if (c >= 2 && !wait1(&bar.empty[tile][st], ((c >> 1) & 1) ^ 1)) return false;
+#pragma unroll 1
+        for (int i = 0; i < 3 && ok; ++i) {
+          const int tile = c == 1 ? (i + 1) % 3 : i;
+          if (!FULL && tile == kTileQ) continue;
+          const int stages = tile == kTileQ ? 1 : 2, st = c & (stages - 1);
+          const int blocks = tile == kTileV ? BV / 64 : DK / 64;
+          const int x = tile == kTileV ? vb * BV : 0, head = tile == kTileV ? h : hq;
+          const CUtensorMap* map = tile == kTileQ ? &map_q : tile == kTileK ? &map_k : &map_v;
+          unsigned char* to = smem + (tile == kTileQ ? L::kQ : st * L::kStage + (tile == kTileK ? L::kK : L::kV));
+          if (c >= stages && !(ok = wait1(&bar.empty[tile][st], (c / stages - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.full[tile][st], blocks * kTile);
-          for (int b = 0; b < blocks; ++b)
-            tc::tma_load_4d(stage + at + b * kTile, map, x + b * 64, head, t, batch, &bar.full[tile][st]);
+          for (int b = 0; b < blocks; ++b) tc::tma_load_4d(to + b * kTile, map, x + b * 64, head, t, batch, &bar.full[tile][st]);
           armed[tile] = c + 1;
-          return true;
-        };
-        ok = (!FULL || load(kTileQ, &map_q, L::kQ, DK / 64, 0, hq)) && load(kTileV, &map_v, L::kV, BV / 64, vb * BV, h) &&
-             load(kTileK, &map_k, L::kK, DK / 64, 0, hq);
+        }
       }
       // no copy may be in flight when the shared memory is released
 #pragma unroll
-      for (int tile = 0; tile < 3; ++tile)
-        for (int j = max(0, armed[tile] - 2); j < armed[tile]; ++j)
-          if (!wait1(&bar.full[tile][j & 1], (j >> 1) & 1)) ok = false;
+      for (int tile = 0; tile < 3; ++tile) {
+        const int stages = tile == kTileQ ? 1 : 2;
+        for (int j = max(0, armed[tile] - stages); j < armed[tile]; ++j)
+          if (!wait1(&bar.full[tile][j & (stages - 1)], (j / stages) & 1)) ok = false;
+      }
     }
   } else if (warp == kWarpGate) {
     // ------------------------------------------------ gates: 4 tokens per lane
@@ -740,13 +764,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (FULL && warp == kWarpStore) {
     if (tc::elect_one()) {  // whole chunks of O leave by TMA; V writes a short one
       for (int c = 0; c < chunks && seq.len - c * kC >= kC; ++c) {
-        const int st = c & 1;
         if (!(ok = wait1(&bar.o_staged, c & 1))) break;
         for (int b = 0; b < BV / 64; ++b)
-          tc::tma_store_4d(&map_o, smem + st * L::kStage + L::kO + b * kTile, vb * BV + b * 64, h, seq.start + c * kC, batch);
+          tc::tma_store_4d(&map_o, smem + L::kO + b * kTile, vb * BV + b * 64, h, seq.start + c * kC, batch);
         bulk_commit();
         bulk_wait_read();
-        mbar_arrive(L::kOInK ? &bar.empty[kTileK][st] : &bar.empty[kTileV][st]);
+        mbar_arrive(&bar.o_stored);
       }
       bulk_wait_all();
     }
@@ -804,6 +827,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       add_ds(1);
       tc::commit(&bar.v_free[1]);
       tc::commit(&bar.ds_done);
+      tc::commit(&bar.empty[kTileK][st]);
 
       if constexpr (FULL) {
         ok = wait1(&bar.p_ready, c & 1);
@@ -813,11 +837,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kC / 16; ++s)
           tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
         tc::commit(&bar.pv_done);
-        tc::commit(L::kOInK ? &bar.empty[kTileV][st] : &bar.empty[kTileK][st]);
-      } else {
-        tc::commit(&bar.empty[kTileV][st]);
-        tc::commit(&bar.empty[kTileK][st]);
       }
+      tc::commit(&bar.empty[kTileV][st]);
     }
     if (!ok) {  // products in flight end before the tensor memory is released
       tc::commit(&bar.drain);
