@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           lds64(w + tb * 8, ww[tb]);
           lds64(w + tb * 8 + 4, ww[tb] + 2);
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 2; ++i) {
           const int dv = quarter * 32 + i * 16;  // of this warp's 16 rows
           const uint32_t block = tile + (dv >> 6) * kTile;
@@ -677,25 +677,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kWarpGate) {
     // ------------------------------------------------ gates: 4 tokens per lane
-    const int64_t g0 = batch * a.g_sb + h * a.g_sh;
-    float x[4], next[4], sum = 0.f;
+    const bool wide = a.g_dtype == GDN_DT_F32;
+    const int64_t step = a.g_st * (wide ? 4 : 2);
+    const char* at = static_cast<const char*>(a.g) + (batch * a.g_sb + h * a.g_sh) * (wide ? 4 : 2) +
+                     (seq.start + lane * 4) * step;
+    uint32_t next[4] = {0, 0, 0, 0};
+    float x[4], sum = 0.f;
 #pragma unroll 1
     for (int c = -1; c < chunks; ++c) {  // a chunk's gates are fetched while the one before is at work
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = next[e];
-        const int t = (c + 1) * kC + lane * 4 + e;
-        next[e] = t < seq.len ? load_any(a.g, g0 + static_cast<int64_t>(seq.start + t) * a.g_st, a.g_dtype) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        x[e] = log2_gate(wide                         ? __uint_as_float(next[e])
+                         : a.g_dtype == GDN_DT_BF16 ? __uint_as_float(next[e] << 16)
+                                                      : __half2float(__ushort_as_half(static_cast<unsigned short>(next[e]))));
+      const int left = seq.len - (c + 1) * kC - lane * 4;  // of this lane's tokens of the next chunk
+      if (wide) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[e] = e < left ? __ldg(reinterpret_cast<const uint32_t*>(at + e * step)) : 0;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) next[e] = e < left ? __ldg(reinterpret_cast<const uint16_t*>(at + e * step)) : 0;
       }
+      at += kC * step;
       if (c < 0) continue;
       const int st = c & 1;
       float* G = reinterpret_cast<float*>(smem + L::kGate + st * L::kGateStage);
       // G summed from the front; the weights' exponents from the back, so that those
       // near zero are sums of few small numbers and keep their precision
       float fwd[4], bwd[4];
-      fwd[0] = x[0] = log2_gate(x[0]);
+      fwd[0] = x[0];
 #pragma unroll
-      for (int e = 1; e < 4; ++e) fwd[e] = fwd[e - 1] + (x[e] = log2_gate(x[e]));
+      for (int e = 1; e < 4; ++e) fwd[e] = fwd[e - 1] + x[e];
       bwd[3] = 0.f;
 #pragma unroll
       for (int e = 2; e >= 0; --e) bwd[e] = bwd[e + 1] + x[e + 1];
