@@ -886,12 +886,24 @@ __global__ void __launch_bounds__(256) lin_scan_kernel(const __grid_constant__ P
     S = *reinterpret_cast<const float4*>(a.initial_state + s.page * a.initial_sp + e);
   float* slot = p.slot_state + first * page + e;
   *reinterpret_cast<float4*>(slot) = S;
-  for (int j = 0; j + 1 < count; ++j) {
-    slot += page;
-    const float4 x = *reinterpret_cast<const float4*>(slot);
-    const float d = p.decay[static_cast<int64_t>(first + j) * a.Hv + h];
-    S = make_float4(fmaf(d, S.x, x.x), fmaf(d, S.y, x.y), fmaf(d, S.z, x.z), fmaf(d, S.w, x.w));
-    *reinterpret_cast<float4*>(slot) = S;
+  // eight slots at a time: the loads do not wait for one another
+  for (int j0 = 0; j0 + 1 < count; j0 += 8) {
+    float4 x[8];
+    float d[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + i;
+      if (j + 1 >= count) break;
+      x[i] = *reinterpret_cast<const float4*>(slot + (j + 1) * page);
+      d[i] = p.decay[static_cast<int64_t>(first + j) * a.Hv + h];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int j = j0 + i;
+      if (j + 1 >= count) break;
+      S = make_float4(fmaf(d[i], S.x, x[i].x), fmaf(d[i], S.y, x[i].y), fmaf(d[i], S.z, x[i].z), fmaf(d[i], S.w, x[i].w));
+      *reinterpret_cast<float4*>(slot + (j + 1) * page) = S;
+    }
   }
 }
 
@@ -948,13 +960,13 @@ Cut choose_cut(const lin_prefill_args_t& a, int sms) {
   } else {
     // Cost in chunks of time, kStart of them to start a CTA, a piece's state pass
     // kState of a whole one, kScan for the scan and the launches (measured, d = 128).
-    constexpr double kStart = 2.0, kState = 0.5, kScan = 4.0;
+    constexpr double kStart = 2.0, kState = 0.5, kScan = 3.0;
     const auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
-    double best = waves(rows * a.B) * (chunks + kStart);
+    double best = 0.95 * waves(rows * a.B) * (chunks + kStart);
     for (int m = 2; m <= 32 && m <= chunks / 4; ++m) {
       const int64_t len = (chunks + m - 1) / m, used = (chunks + len - 1) / len;
       const double cost = waves(rows * a.B * used) * (len + kStart) + waves(rows * a.B * (used - 1)) * (kState * len + kStart) + kScan;
-      if (cost < 0.95 * best) {
+      if (cost < best) {
         best = cost;
         cut.piece = static_cast<int>(len * kC);
         cut.pieces = static_cast<int>(used);
