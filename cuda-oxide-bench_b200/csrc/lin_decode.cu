@@ -7,11 +7,12 @@
 // flops), so the kernel is bound by HBM; q, k, v and o are 1/100 of that.
 //
 // Unlike the delta rule nothing has to be reduced before the state can be
-// written back: S' = a S + k v^T is elementwise, and o = a q^T S + (q.k) v is
-// summed on the side.  So there is no ring and no producer warp: a CTA takes
-// one DK x BV slab of a head's state (columns are independent), every thread
-// issues the loads of all its rows at once, and the CTAs resident on an SM
-// hide each other's latency.
+// written back: S' = a S + k v^T is elementwise, and o = q^T S' is summed on the
+// side.  So there is no ring and no producer warp: a CTA takes one DK x BV slab of
+// a head's state (columns are independent), every thread issues the loads of all
+// its rows at once, and the CTAs resident on an SM hide each other's latency.
+// B = 1024, H = 32, d = 128: 641 us, 6.7 TB/s of state, the measured copy's rate and
+// what the GDN decode's ring reaches; with pages in random order 5% less.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -183,6 +184,7 @@ int validate(const lin_decode_args_t* a) {
       !stride_ok(a->v_sb, 2) || !stride_ok(a->v_sh, 2) || !stride_ok(a->o_sb, 2) || !stride_ok(a->o_sh, 2) ||
       !stride_ok(a->state_in_sp, 4) || !stride_ok(a->state_out_sp, 4))
     return GDN_ERR_ALIGN;
+  if ((a->B > 1 && a->o_sb == 0) || (a->Hv > 1 && a->o_sh == 0)) return GDN_ERR_SHAPE;  // rows of o on one another
   if (a->state_in != a->state_out) {
     const float *i1 = a->state_in + (a->pages - 1) * a->state_in_sp + page;
     const float *o1 = a->state_out + (a->pages - 1) * a->state_out_sp + page;

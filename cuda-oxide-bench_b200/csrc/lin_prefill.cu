@@ -12,24 +12,38 @@
 // everything else pipelines.  One CTA takes one sequence, value head and block
 // of BV value columns (columns are independent) through all its chunks, so q,
 // k, v and o cross HBM once and the state stays on chip.  Per chunk of d = 128
-// that is 128 KB against five 128^3 products.
+// that is 128 KB against five 128^3 products (one more than the formulas have:
+// the state's increment is two, see V'').  C = 128 and not 64: the state's update
+// and its rounding to an operand cost the same per chunk, whatever its length.
 //
-// Warps (19): R 0-3 (a row of the chunk per thread), V 4-7, S 8-15, TMA 16,
-// gates 17, MMA 18.  Per chunk, in the MMA warp's order:
-//   SC  scores = Q K^T             Q in TMEM (R); R turns them into
-//                                  P, packed over the scores' own columns
+// Warps (20): R 0-3 (a row of the chunk per thread), V 4-7, S 8-15, TMA loads 16,
+// gates 17, MMA 18, TMA stores 19.  Per chunk, in the MMA warp's order:
+//   SC  scores = Q K^T             Q copied into TMEM by R, which then turns the
+//                                  scores into P, packed over their own columns
 //   D0  dS^T  = V''^T K            of the chunk's first 64 tokens, V'' in TMEM (V)
 //   QS  O     = Q S                S^T in shared memory
 //   D1  dS^T += V''^T K            of the others; then S reads dS and rewrites S^T
-//   PV  O    += P V                then S writes O out
-// All five take A from TMEM: a product with both operands in shared memory
-// reads it at its full rate, and other warps' reads then take five times as
-// long (4 ldmatrix.x4: 726 cycles against 141).
+//   PV  O    += P V                then V applies the rows' factors and stages O
+// D0 and D1 lie between the others so that the tensor cores have work while R and
+// V prepare the next operand.  All five take A from TMEM: a product with both
+// operands in shared memory reads it at its full rate, and other warps' reads then
+// take five times as long (4 ldmatrix.x4: 726 cycles against 141).
+//
 // V'' = w v, w = e^(G_C - G_j), is split into two parts of the I/O type, hi +
 // lo, because the state is kept to fp32 accuracy: one part would leave half a
-// step of the I/O type of every term.  So is w, which makes both parts a few
-// packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo = (v w_hi -
-// hi) + v w_lo, the difference being exact.
+// step of the I/O type of every term (2^-8 in bf16).  So is w, which makes both
+// parts a few packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo =
+// (v w_hi - hi) + v w_lo, the difference being exact.  Against 64 bits the state is
+// off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
+// state that QS takes, each rounded to bf16 once, give the rest).
+//
+// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 122 us, 403 MB, so
+// 3.3 TB/s or 0.51 of the measured copy): a CTA takes 4700 cycles a chunk.  The
+// tensor pipe is busy for 0.47 of them; shared memory moves about 3900 of the 4700
+// x 128 bytes it could (operands 1280, TMA 1000, the warps' 1600); and instruction
+// fetch: five roles of straight-line code pass through the SM's instruction cache
+// once a chunk, at 0.89 hits.  So loops are kept rolled and call sites single where
+// that is possible; unrolled, the same kernel took 226 us.
 #include <cuda_runtime.h>
 
 #include <atomic>
@@ -61,8 +75,8 @@ enum { kNearMid = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
-constexpr uint32_t kTmQ = 128;    // Q' bf16 [DK / 2]
-constexpr uint32_t kTmV = 192;    // V'' [64]
+constexpr uint32_t kTmQ = 128;    // Q, or Q' in bf16 [DK / 2]
+constexpr uint32_t kTmV = 192;    // V'': lo [32], hi [32] of 64 tokens
 constexpr uint32_t kTmO = 256;    // O fp32 [BV]
 constexpr uint32_t kTmDS = 384;   // dS^T fp32 [DK]
 
@@ -958,8 +972,11 @@ Cut choose_cut(const lin_prefill_args_t& a, int sms) {
     cut.piece = static_cast<int>(most * kC);
     cut.slots = 2 * (static_cast<int64_t>(a.T) / cut.piece);
   } else {
-    // Cost in chunks of time, kStart of them to start a CTA, a piece's state pass
-    // kState of a whole one, kScan for the scan and the launches (measured, d = 128).
+    // Cost in chunks of time (2.5 us), kStart of them to start a CTA, a piece's state
+    // pass kState of a whole one, kScan for the scan and the launches.  Measured, d =
+    // 128, one sequence: 32 heads, 32768 tokens 700 us whole, 317 in 9 pieces (345 in
+    // 4, 401 in 7); 8 heads 95 in 18 (146 in 9); 32 heads, 4096 tokens 55 in 4 (70 in 9);
+    // two sequences of 8192 (64 CTAs) 172 to 185 in 2 and 190 in 4.
     constexpr double kStart = 2.0, kState = 0.5, kScan = 3.0;
     const auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
     double best = 0.95 * waves(rows * a.B) * (chunks + kStart);

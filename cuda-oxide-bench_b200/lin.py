@@ -34,7 +34,12 @@ def _on(first, *others) -> int:
 
 def _status(dev: int) -> int:
     w = _status_words.get(dev)
-    return (status_word(dev) if w is None else w).data_ptr()
+    if w is None:
+        if torch.cuda.is_current_stream_capturing():
+            # the word outlives any graph, so it cannot come from a graph's memory
+            raise GDNError(f"the first call on cuda:{dev} cannot be captured: call once before", 2)
+        w = status_word(dev)
+    return w.data_ptr()
 
 
 def _launch(fn, args, dev: int, what: str) -> None:
@@ -96,7 +101,8 @@ def lin_decode(q, k, v, g, state, *, scale: float = 1.0, out=None, gate: str = "
     row b uses page index[b].  A negative index is an idle row: its output is
     zero and no state is touched.  An index >= P, or one that an earlier row
     holds, is treated as idle and reported (``check=True`` synchronises and
-    raises).  Rows without a page leave ``state_out`` as it was.
+    raises).  Rows without a page leave ``state_out`` as it was.  ``out`` must
+    not share memory with the inputs.
     """
     dev = _on(q, k, v, g, state, state_out, out, index)
     if out is None:
@@ -165,7 +171,13 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
     zero and keeps no state.  Indices out of range or taken by an earlier
     sequence, and offsets that are out of range or descend, are reported
     (``check=True``).  q, k, v and out may be strided views whose rows are
-    contiguous and 16-byte aligned.
+    contiguous and 16-byte aligned; out must not share memory with them.
+
+    Few heads and a long T: the time axis is cut, with a workspace from torch's
+    allocator (or ``workspace``, at least as large).  Infinities and NaN in a row
+    can reach the rows up to 127 before it in its sequence (they share a chunk),
+    never another sequence.  f16: P = q.k e^(G_i - G_j) scale and e^(G_C - G_j) v
+    have to stay below 65504, which only large values or growing gates pass.
     """
     dev = _on(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, workspace)
     if out is None:

@@ -62,6 +62,7 @@ def decode_args(pkg, **over):
     ({"state_out": BASE + 4 * (1 << 32) + 4096}, 2),
     ({"io_dtype": 0}, 4), ({"g_dtype": 7}, 4), ({"gate_kind": 5}, 4),
     ({"q": BASE + 8}, 3), ({"v_sh": 100}, 3), ({"state_in_sp": 4 * 128 * 128 + 2}, 3),
+    ({"o_sb": 0}, 2), ({"o_sh": 0}, 2),
 ])
 def test_decode_refuses(pkg, over, code):
     a = decode_args(pkg, **over)
@@ -89,7 +90,7 @@ def prefill_args(pkg, **over):
 @pytest.mark.parametrize("over,code", [
     ({"k": 0}, 1), ({"final_state": 0}, 1),
     ({"Hqk": 3}, 2), ({"dk": 256}, 2), ({"dv": 32}, 2), ({"T": 0}, 2), ({"B": 0}, 2), ({"B": 70000}, 2),
-    ({"pages": 1}, 2), ({"final_sp": 64}, 2), ({"q_st": -256}, 2),
+    ({"pages": 1}, 2), ({"final_sp": 64}, 2), ({"q_st": -256}, 2), ({"o_st": 0}, 2), ({"k_sh": 0}, 2),
     ({"initial_state": BASE + 4 * (1 << 32) + 64}, 2),
     ({"initial_state": BASE + 4 * (1 << 32), "initial_sp": 5 * 128 * 128}, 2),
     ({"io_dtype": 0}, 4), ({"g_dtype": -1}, 4),

@@ -212,10 +212,11 @@ def test_prefill_gate_ranges(pkg, io, gmin, gmax):
                   k[0], v[0])
 
 
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("g_reset", [float("-inf"), -200.0, -1e30])
-def test_prefill_resets(pkg, g_reset):
+def test_prefill_resets(pkg, g_reset, io):
     """A decay of zero at some tokens starts the sequence anew there, also inside a chunk."""
-    T, d, io = 260, 64, torch.bfloat16
+    T, d = 260, 64
     q, k, v, g = make((1, T), 1, 2, d, d, io, 10)
     g[0, [0, 5, 6, 127, 128, 200], 0] = g_reset
     g[0, :, 1] = g_reset
@@ -386,6 +387,41 @@ def test_prefill_packed_unsound_offsets_of_long_sequences(pkg):
     with pytest.raises(pkg.GDNError, match="index"):
         pkg.lin_prefill(q, k, v, g, final_state=fin, cu_seqlens=cu, check=True)
     assert bool((fin[[1, 3]] == 3).all())
+
+
+def test_prefill_workspace_argument(pkg):
+    q, k, v, g = (x.to(DEV) for x in make((1, 4096), 1, 1, 64, 64, torch.bfloat16, 34))
+    want = pkg.lin_prefill(q, k, v, g, check=True)
+    with pytest.raises(pkg.GDNError, match="workspace"):
+        pkg.lin_prefill(q, k, v, g, workspace=torch.empty(64, dtype=torch.uint8, device=DEV))
+    ws = torch.full((1 << 22,), 255, dtype=torch.uint8, device=DEV)  # whatever it holds before
+    got = pkg.lin_prefill(q, k, v, g, workspace=ws, check=True)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_prefill_repeats_to_the_bit(pkg):
+    x = [t.to(DEV) for t in make((2, 1500), 2, 4, 128, 128, torch.bfloat16, 35)]
+    first = pkg.lin_prefill(*x, check=True)
+    for _ in range(3):
+        again = pkg.lin_prefill(*x)
+        assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+def test_two_streams_at_once(pkg):
+    """Two cut prefills in flight together: each has a workspace of its own."""
+    sets = [[t.to(DEV) for t in make((1, 6000), 1, 2, 64, 64, torch.bfloat16, s)] for s in (36, 37)]
+    want = [pkg.lin_prefill(*x, check=True) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(3):
+        for x, st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                got.append(pkg.lin_prefill(*x))
+    torch.cuda.synchronize()
+    for i, (o, S) in enumerate(got):
+        assert torch.equal(o, want[i % 2][0]) and torch.equal(S, want[i % 2][1])
+    pkg.check_device_status(torch.device(DEV))
 
 
 def test_graph_capture_on_another_stream(pkg):
