@@ -152,12 +152,15 @@ __device__ __forceinline__ void find_rows(const lin_prefill_args_t& a, int n, Se
 // sequence is none (-1).
 __device__ Seq find_seq(const lin_prefill_args_t& a, int n, bool reporter) {
   Seq s;
+  s.page = a.index ? a.index[n] : n;
+  // the first of the earlier pages, asked for together with this one's
+  const int j0 = threadIdx.x;
+  const int other = a.index && j0 < n ? a.index[j0] : -1;
   find_rows(a, n, s);
   bool bad = s.len < 0;
-  s.page = a.index ? a.index[n] : n;
-  bool taken = s.page >= a.pages;
+  bool taken = s.page >= a.pages || (other >= 0 && other == s.page);
   if (a.index && s.page >= 0)
-    for (int j = threadIdx.x; j < n; j += blockDim.x) taken |= a.index[j] == s.page;
+    for (int j = j0 + blockDim.x; j < n; j += blockDim.x) taken |= a.index[j] == s.page;
   if (__syncthreads_or(taken)) {
     bad = true;
     s.page = -1;
@@ -323,14 +326,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const lin_prefill_args_t& a = p.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int h = blockIdx.x / p.nvb, vb = blockIdx.x - h * p.nvb, hq = h / (a.Hv / a.Hqk);
-  pdl_launch_dependents();
-  pdl_wait();
-  const Item seq = find_item<FULL>(p, blockIdx.y, FULL && blockIdx.x == 0 && tid == 0);
-  if (seq.len < 0) return;
-  const int chunks = (seq.len + kC - 1) / kC;
-  const int batch = a.cu_seqlens ? 0 : p.piece && static_cast<int>(blockIdx.y) < p.slots ? blockIdx.y / p.pieces
-                                    : blockIdx.y - (p.piece ? p.slots : 0);
-
   if (warp == kWarpMma) tc::tmem_alloc(&bar.tmem, 512);
   if (tid == 0) {
     for (int s = 0; s < 2; ++s) {
@@ -359,6 +354,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.drain, 1);
     fence_mbar_init();
   }
+  if (tid < 4) prefetch_map(tid == 0 ? &map_q : tid == 1 ? &map_k : tid == 2 ? &map_v : &map_o);
+  pdl_launch_dependents();
+  pdl_wait();
+  // (a CTA without work goes through the roles with no chunks and no state)
+  const Item seq = find_item<FULL>(p, blockIdx.y, FULL && blockIdx.x == 0 && tid == 0);
+  const int chunks = seq.len > 0 ? (seq.len + kC - 1) / kC : 0;
+  const int batch = a.cu_seqlens ? 0 : p.piece && static_cast<int>(blockIdx.y) < p.slots ? blockIdx.y / p.pieces
+                                    : blockIdx.y - (p.piece ? p.slots : 0);
   tc::fence_before_sync();
   __syncthreads();
   tc::fence_after_sync();
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.gfull[st]);
     }
-    if (!FULL && lane == 0 && vb == 0) p.decay[static_cast<int64_t>(blockIdx.y) * a.Hv + h] = ex2(sum);
+    if (!FULL && lane == 0 && vb == 0 && chunks) p.decay[static_cast<int64_t>(blockIdx.y) * a.Hv + h] = ex2(sum);
   } else if (FULL && warp == kWarpStore) {
     if (tc::elect_one()) {  // whole chunks of O leave by TMA; V writes a short one
       for (int c = 0; c < chunks && seq.len - c * kC >= kC; ++c) {
@@ -968,7 +971,8 @@ Cut choose_cut(const lin_prefill_args_t& a, int sms) {
     // more than half of the time that the whole work takes, and 2048 tokens at least.
     const int64_t share = (chunks * rows + 2 * sms - 1) / (2 * sms);
     const int64_t most = share > 16 ? share : 16;
-    if (chunks < 4 * most) return cut;
+    // (with many sequences a long one has others beside it)
+    if (chunks < (rows * a.B < 4 * sms ? 4 : 8) * most) return cut;
     cut.piece = static_cast<int>(most * kC);
     cut.slots = 2 * (static_cast<int64_t>(a.T) / cut.piece);
   } else {

@@ -162,6 +162,11 @@ __device__ __forceinline__ void bulk_wait_all() {
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
+// Brings a tensor map (a kernel parameter) into the cache its copies read it from.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
 // 2-D tiled TMA load (no multicast) of the box at (x = column, y = row) of
 // `map` into shared memory, completing on an mbarrier.  x * element size must
 // be a multiple of 16 bytes.
