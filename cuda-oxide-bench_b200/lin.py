@@ -54,12 +54,14 @@ def _launch(fn, args, dev: int, what: str) -> None:
         _lib.check(rc, what)
 
 
-def _check_io(q, k, v, out) -> None:
+def _check_io(q, k, v, out) -> int:
+    """q's element type, which k, v and out share."""
     dt = q.dtype
     if k.dtype is not dt or v.dtype is not dt or out.dtype is not dt:
         raise GDNError("q, k, v and out must share one dtype (bf16 or f16)", 4)
     if out.shape != v.shape:
         raise GDNError(f"out must have the shape of v, {tuple(v.shape)}, got {tuple(out.shape)}", 2)
+    return _dt(q, "q")
 
 
 def _check_rows(**strides) -> None:
@@ -123,7 +125,7 @@ def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate,
         raise GDNError("q, k must be [B, Hqk, d_k] and v [B, Hv, d_v]", 2)
     B, Hqk, dk = shape
     _, Hv, dv = v_shape
-    _check_io(q, k, v, out)
+    io = _check_io(q, k, v, out)
     qs, ks, vs, os, gs = q.stride(), k.stride(), v.stride(), out.stride(), g.stride()
     if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os[2] != 1:
         _check_rows(q=qs, k=ks, v=vs, out=os)
@@ -146,7 +148,7 @@ def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate,
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(),
         state_out.data_ptr(), out.data_ptr(), None if index is None else index.data_ptr(),
         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], g_sb, g_sh, in_sp, out_sp,
-        B, Hqk, Hv, dk, dv, pages, _dt(q, "q"), _dt(g, "g"), _LOG if gate == "log" else _LINEAR,
+        B, Hqk, Hv, dk, dv, pages, io, _dt(g, "g"), _LOG if gate == "log" else _LINEAR,
         scale, status)
 
 
@@ -216,7 +218,7 @@ def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index
         raise GDNError("q, k must be [B, T, Hqk, d_k] and v [B, T, Hv, d_v]", 2)
     B, T, Hqk, dk = shape
     _, _, Hv, dv = v_shape
-    _check_io(q, k, v, out)
+    io = _check_io(q, k, v, out)
     qs, ks, vs, os, gs = q.stride(), k.stride(), v.stride(), out.stride(), g.stride()
     if qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or os[3] != 1:
         _check_rows(q=qs, k=ks, v=vs, out=os)
@@ -245,4 +247,4 @@ def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index
         out.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
         None if index is None else index.data_ptr(),
         *qs[:3], *ks[:3], *vs[:3], *os[:3], *gs, in_sp, fin_sp,
-        seqs, T, Hqk, Hv, dk, dv, pages, _dt(q, "q"), _dt(g, "g"), scale, None, 0, status)
+        seqs, T, Hqk, Hv, dk, dv, pages, io, _dt(g, "g"), scale, None, 0, status)
