@@ -417,8 +417,9 @@ int lin_decode_launch(const lin_decode_args_t* args, gdn_stream_t stream);
  * state in the same page of final_state, which may equal initial_state or be
  * disjoint from it.  A sequence with a negative index starts from zero and
  * its state is not kept; one of no tokens keeps its initial state.
- * d_k in {64, 128}, d_v a multiple of 64.  Strides as for the decode step.
- * Log gates only.  Workspace: lin_prefill_workspace_size(args) bytes (0 for
+ * d_k in {64, 128}, d_v a multiple of 64.  Strides as for the decode step, and
+ * positive on every axis of more than one entry (g's may be 0).  o must not
+ * share memory with q, k or v.  Log gates only.  Workspace: lin_prefill_workspace_size(args) bytes (0 for
  * many shapes), 16-byte aligned, owned by the caller.
  */
 typedef struct {

@@ -135,6 +135,17 @@ def test_decode_strides_out_of_place_and_pool_slices(pkg):
                  torch.bfloat16)
 
 
+def test_decode_more_rows_than_a_grid_axis(pkg):
+    B, d = 66000, 64
+    q, k, v, g = make((B,), 1, 1, d, d, torch.bfloat16, 38)
+    S = torch.randn(1, 1, d, d, generator=torch.Generator().manual_seed(39))
+    st = S.to(DEV).repeat(B, 1, 1, 1)
+    o = pkg.lin_decode(*(x.to(DEV) for x in (q, k, v, g)), st, check=True)
+    rows = [0, 1, 65534, 65535, 65536, B - 1]
+    check_decode(o[rows].cpu(), st[rows].cpu(), q[rows], k[rows], v[rows], g[rows], S.expand(len(rows), -1, -1, -1), 1.0,
+                 torch.bfloat16)
+
+
 def test_decode_large_pool_offsets(pkg):
     """Pages whose element offsets pass 32 bits."""
     if torch.cuda.mem_get_info()[0] < 24 << 30:
@@ -351,6 +362,22 @@ def test_prefill_long_in_place(pkg, T, io):
     for b in range(B):
         ref = steps(q[b], k[b], v[b], g[b], S0[b], 0.1)
         check_prefill(o[b].cpu(), fin[b].cpu(), ref, io, k[b], v[b])
+
+
+def test_prefill_long_with_pages_of_layers(pkg):
+    """A cut dense batch whose states are pages of one layer of a larger pool."""
+    B, T, H, d, io = 2, 2500, 2, 64, torch.bfloat16
+    q, k, v, g = make((B, T), H, H, d, d, io, 40, gmin=-0.02)
+    pool = torch.randn(5, 3, H, d, d, generator=torch.Generator().manual_seed(41))
+    st, index = pool.to(DEV), torch.tensor([4, 1], dtype=torch.int32)
+    o, fin = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st[:, 1], scale=0.1, index=index.to(DEV), check=True)
+    st = st.cpu()
+    for b in range(B):
+        p = int(index[b])
+        ref = steps(q[b], k[b], v[b], g[b], pool[p, 1], 0.1)
+        check_prefill(o[b].cpu(), st[p, 1], ref, io, k[b], v[b])
+        pool[p, 1] = st[p, 1]
+    assert torch.equal(st, pool)  # nothing else was written
 
 
 def test_prefill_packed_long_and_short(pkg):
