@@ -7,6 +7,7 @@ implementation.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -177,6 +178,36 @@ class PagesArgs(ctypes.Structure):
         (ctypes.c_size_t, "workspace_bytes"),
         (_vp, "status"),
     )
+
+
+class Packed:
+    """An argument struct as bytes, with the function that takes it: filling a
+    ctypes structure field by field is three times as slow, which shows in a call
+    that takes 5 us on the GPU.  ``pack(*values)`` takes a value per field, 0 for
+    NULL; ``call(bytes, stream)`` runs the function."""
+
+    _CODES = {ctypes.c_void_p: "P", ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f",
+              ctypes.c_size_t: "N", ctypes.POINTER(PagesPool): "P"}
+
+    def __init__(self, cls, function: str):
+        fmt = "".join(self._CODES[t] for _, t in cls._fields_)
+        # native alignment, and the structure's own padding at its end
+        self._struct = struct.Struct("@" + fmt + "0P")
+        assert self._struct.size == ctypes.sizeof(cls), function
+        self._function, self._call = function, None
+
+    def pack(self, *values) -> bytes:
+        try:
+            return self._struct.pack(*values)
+        except (OverflowError, struct.error) as e:  # a size past 32 bits
+            raise GDNError(f"{self._function}: {e}", 1) from None
+
+    @property
+    def call(self):
+        if self._call is None:
+            proto = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
+            self._call = proto((self._function, load()))
+        return self._call
 
 
 _lock = threading.Lock()

@@ -90,31 +90,6 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-// Same for kernels in which many warps wait while others compute: a waiting
-// thread sleeps in the barrier unit for up to 100 us at a time instead of
-// polling, and the limit (about a second) is counted in such sleeps and in the
-// SM's own cycles, so that waiting takes no issue slots and no reads of the
-// device-wide timer.
-__device__ __forceinline__ bool mbar_wait_asleep(uint64_t* bar, uint32_t parity) {
-  constexpr long long kLimit = 2000ll * 1000ll * 1000ll;
-  const auto asleep = [&] {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
-        : "memory");
-    return ok != 0;
-  };
-  if (asleep()) return true;
-  const long long t0 = clock64();
-  while (!asleep())
-    if (clock64() - t0 > kLimit) return false;
-  return true;
-}
-
 // Named barrier over `count` threads that also ORs a predicate across them.
 __device__ __forceinline__ bool named_barrier_or(int id, int count, bool pred) {
   uint32_t r;

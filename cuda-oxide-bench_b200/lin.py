@@ -18,6 +18,9 @@ from .api import _dt, _status_words, check_device_status, status_word
 # the current stream's handle without a Stream object around it (1.2 us less per call)
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
     else lambda dev: torch.cuda.current_stream(dev).cuda_stream
+_DECODE = _lib.Packed(_lib.LinDecodeArgs, "lin_decode_launch")
+_PREFILL = _lib.Packed(_lib.LinPrefillArgs, "lin_prefill_launch")
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _LOG, _LINEAR = _lib.GATE_LOG, _lib.GATE_LINEAR
 
 
@@ -42,14 +45,19 @@ def _status(dev: int) -> int:
     return w.data_ptr()
 
 
-def _launch(fn, args, dev: int, what: str) -> None:
+def _check_scale(scale) -> None:
+    if not -_FLOAT_MAX <= scale <= _FLOAT_MAX:
+        raise GDNError(f"scale must be a finite float, got {scale}", 2)
+
+
+def _launch(packed, args: bytes, dev: int, what: str) -> None:
     """Calls a launcher on the tensors' device and that device's current stream."""
     stream = _raw_stream(dev)
     if torch.cuda.current_device() == dev:
-        rc = fn(ctypes.byref(args), stream)
+        rc = packed.call(args, stream)
     else:
         with torch.cuda.device(dev):
-            rc = fn(ctypes.byref(args), stream)
+            rc = packed.call(args, stream)
     if rc:
         _lib.check(rc, what)
 
@@ -112,14 +120,14 @@ def lin_decode(q, k, v, g, state, *, scale: float = 1.0, out=None, gate: str = "
     if state_out is None:
         state_out = state
     a = _decode_args(q, k, v, g, state, state_out, out, index, scale, gate, _status(dev))
-    _launch(_lib.load().lin_decode_launch, a, dev, "lin_decode")
+    _launch(_DECODE, a, dev, "lin_decode")
     if check:
         check_device_status(dev)
     return out
 
 
 def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate,
-                 status=None) -> _lib.LinDecodeArgs:
+                 status=0) -> bytes:
     shape, v_shape = q.shape, v.shape
     if len(shape) != 3 or k.shape != shape or len(v_shape) != 3 or v_shape[0] != shape[0]:
         raise GDNError("q, k must be [B, Hqk, d_k] and v [B, Hv, d_v]", 2)
@@ -144,9 +152,10 @@ def _decode_args(q, k, v, g, state, state_out, out, index, scale, gate,
         if state_out.shape[0] != pages:
             raise GDNError("state_out must have as many pages as state", 2)
     _check_index(index, B, pages)
-    return _lib.LinDecodeArgs(
+    _check_scale(scale)
+    return _DECODE.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), state.data_ptr(),
-        state_out.data_ptr(), out.data_ptr(), None if index is None else index.data_ptr(),
+        state_out.data_ptr(), out.data_ptr(), 0 if index is None else index.data_ptr(),
         qs[0], qs[1], ks[0], ks[1], vs[0], vs[1], os[0], os[1], g_sb, g_sh, in_sp, out_sp,
         B, Hqk, Hv, dk, dv, pages, io, _dt(g, "g"), _LOG if gate == "log" else _LINEAR,
         scale, status)
@@ -193,10 +202,9 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
             rows = v.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
             final_state = torch.empty((rows, v.shape[2], q.shape[3], v.shape[3]),
                                       dtype=torch.float32, device=q.device)
-    a = _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale,
-                      _status(dev))
-    L = _lib.load()
-    need = L.lin_prefill_workspace_size(ctypes.byref(a))
+    args = (q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale, _status(dev))
+    a = _prefill_args(*args)
+    need = _prefill_workspace(a)
     if need:
         # from the allocator on the current stream, so that calls on other streams
         # and captured graphs have workspaces of their own
@@ -204,15 +212,20 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
         elif not workspace.is_contiguous():
             raise GDNError("workspace must be a contiguous tensor", 2)
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _launch(L.lin_prefill_launch, a, dev, "lin_prefill")
+        a = _prefill_args(*args, workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _launch(_PREFILL, a, dev, "lin_prefill")
     if check:
         check_device_status(dev)
     return out, final_state
 
 
+def _prefill_workspace(args: bytes) -> int:
+    return _lib.load().lin_prefill_workspace_size(
+        ctypes.cast(ctypes.c_char_p(args), ctypes.POINTER(_lib.LinPrefillArgs)))
+
+
 def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale,
-                  status=None) -> _lib.LinPrefillArgs:
+                  status=0, workspace=0, workspace_bytes=0) -> bytes:
     shape, v_shape = q.shape, v.shape
     if len(shape) != 4 or k.shape != shape or len(v_shape) != 4 or v_shape[:2] != shape[:2]:
         raise GDNError("q, k must be [B, T, Hqk, d_k] and v [B, T, Hv, d_v]", 2)
@@ -241,10 +254,12 @@ def _prefill_args(q, k, v, g, initial_state, final_state, out, cu_seqlens, index
         if initial_state.shape[0] != pages:
             raise GDNError("initial_state and final_state must have as many pages", 2)
     _check_index(index, seqs, pages)
-    return _lib.LinPrefillArgs(
+    _check_scale(scale)
+    return _PREFILL.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(),
-        None if initial_state is None else initial_state.data_ptr(), final_state.data_ptr(),
-        out.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-        None if index is None else index.data_ptr(),
+        0 if initial_state is None else initial_state.data_ptr(), final_state.data_ptr(),
+        out.data_ptr(), 0 if cu_seqlens is None else cu_seqlens.data_ptr(),
+        0 if index is None else index.data_ptr(),
         *qs[:3], *ks[:3], *vs[:3], *os[:3], *gs, in_sp, fin_sp,
-        seqs, T, Hqk, Hv, dk, dv, pages, io, _dt(g, "g"), scale, None, 0, status)
+        seqs, T, Hqk, Hv, dk, dv, pages, io, _dt(g, "g"), scale,
+        workspace, workspace_bytes, status)

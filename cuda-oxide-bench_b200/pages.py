@@ -15,6 +15,7 @@ the plain batch that ``gdn_decode`` and ``kda_decode`` take; ``lin_decode`` and
 from __future__ import annotations
 
 import ctypes
+from array import array
 
 import torch
 
@@ -24,11 +25,17 @@ from .api import check_device_status
 from .lin import _launch, _on, _status
 
 
-def _pools(pools) -> tuple[list, "ctypes.Array"]:
+_CALLS = {name: _lib.Packed(_lib.PagesArgs, f"pages_{name}_launch")
+          for name in ("copy", "fork", "free", "compact")}
+_SMALL = 2048  # pages and entries up to which no call needs a workspace
+
+
+def _pools(pools) -> tuple[list, array]:
+    """The pools and their C descriptors (base, page stride, page bytes)."""
     pools = [pools] if isinstance(pools, torch.Tensor) else list(pools)
     if len(pools) > _lib.PAGES_MAX_POOLS:
         raise GDNError(f"at most {_lib.PAGES_MAX_POOLS} pools in a call, got {len(pools)}", 2)
-    flat = []
+    flat = array("q")
     for p in pools:
         if p.dim() < 2 or p.shape[0] != pools[0].shape[0]:
             raise GDNError("pools must be [P, ...] tensors with the same number of pages", 2)
@@ -36,8 +43,8 @@ def _pools(pools) -> tuple[list, "ctypes.Array"]:
         n = p.numel() // P * size if P else 0
         if not p.is_contiguous() and not p[:1].is_contiguous():
             raise GDNError("each page of a pool must be contiguous", 3)
-        flat.append((p.data_ptr(), p.stride(0) * size if P > 1 else n, n))
-    return pools, (_lib.PagesPool * max(1, len(flat)))(*flat)
+        flat.extend((p.data_ptr(), p.stride(0) * size if P > 1 else n, n))
+    return pools, flat
 
 
 def _int32(name: str, t, shape=None) -> None:
@@ -46,22 +53,25 @@ def _int32(name: str, t, shape=None) -> None:
         raise GDNError(f"{name} must be a contiguous int32 [{shape[0] if shape else 'n'}] tensor", 2)
 
 
-def _ptr(t):
-    return None if t is None else t.data_ptr()
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _call(fn: str, like, dev: int, pages: int, *, pools=(), arr=None, used=None, used_out=None, n=0,
+def _call(name: str, like, dev: int, pages: int, *, pools=(), arr=None, used=None, used_out=None, n=0,
           src=None, dst=None, remap=None, count=None, check=False) -> None:
     if not 1 <= pages <= _lib.PAGES_MAX_PAGES:
         raise GDNError(f"a pool must have 1 to {_lib.PAGES_MAX_PAGES} pages, got {pages}", 2)
-    a = _lib.PagesArgs(arr, len(pools), pages, _ptr(used), _ptr(used_out), n, _ptr(src), _ptr(dst),
-                       _ptr(remap), _ptr(count), None, 0, _status(dev))
-    L = _lib.load()
-    need = L.pages_workspace_size(ctypes.byref(a)) if fn != "pages_free_launch" else 0
-    if need:  # from the allocator on the current stream: no two calls in flight share it
-        ws = torch.empty(need, dtype=torch.uint8, device=like.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), need
-    _launch(getattr(L, fn), a, dev, fn.removesuffix("_launch"))
+    packed = _CALLS[name]
+    args = (arr.buffer_info()[0] if pools else 0, len(pools), pages, _ptr(used), _ptr(used_out), n,
+            _ptr(src), _ptr(dst), _ptr(remap), _ptr(count))
+    ws, need, status = 0, 0, _status(dev)
+    if (pages > _SMALL or n > _SMALL) and name != "free":
+        need = _lib.load().pages_workspace_size(ctypes.cast(
+            ctypes.c_char_p(packed.pack(*args, 0, 0, 0)), ctypes.POINTER(_lib.PagesArgs)))
+        # from the allocator on the current stream: no two calls in flight share it
+        buf = torch.empty(need, dtype=torch.uint8, device=like.device)
+        ws = buf.data_ptr()
+    _launch(packed, packed.pack(*args, ws, need, status), dev, f"pages_{name}")
     if check:
         check_device_status(dev)
 
@@ -79,7 +89,7 @@ def pages_copy(pools, src, dst, *, check: bool = False) -> None:
     dev = _on(src, dst, *pools)
     _int32("src", src)
     _int32("dst", dst, tuple(src.shape))
-    _call("pages_copy_launch", src, dev, pools[0].shape[0], pools=pools, arr=arr, n=src.numel(), src=src,
+    _call("copy", src, dev, pools[0].shape[0], pools=pools, arr=arr, n=src.numel(), src=src,
           dst=dst, check=check)
 
 
@@ -114,7 +124,7 @@ def _fork(dev, pools, arr, used, src, n, out, used_out, check):
     _int32("used", used)
     _int32("used_out", used_out, tuple(used.shape))
     _int32("out", out, (n,))
-    _call("pages_fork_launch", used, dev, used.numel(), pools=pools, arr=arr, used=used, used_out=used_out,
+    _call("fork", used, dev, used.numel(), pools=pools, arr=arr, used=used, used_out=used_out,
           n=n, src=src, dst=out, check=check)
     return out
 
@@ -128,7 +138,7 @@ def pages_free(used, index, *, used_out=None, check: bool = False) -> torch.Tens
     _int32("used", used)
     _int32("used_out", used_out, tuple(used.shape))
     _int32("index", index)
-    _call("pages_free_launch", used, dev, used.numel(), used=used, used_out=used_out, n=index.numel(),
+    _call("free", used, dev, used.numel(), used=used, used_out=used_out, n=index.numel(),
           src=index, check=check)
     return used_out
 
@@ -159,6 +169,6 @@ def pages_compact(pools, used, *, index=None, index_out=None, used_out=None, che
         _int32("index_out", index_out, (n,))
     elif index_out is not None:
         raise GDNError("index_out needs index", 1)
-    _call("pages_compact_launch", used, dev, P, pools=pools, arr=arr, used=used, used_out=used_out, n=n,
+    _call("compact", used, dev, P, pools=pools, arr=arr, used=used, used_out=used_out, n=n,
           src=index, dst=index_out, remap=remap, count=count, check=check)
     return remap, count, index_out

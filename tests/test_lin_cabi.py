@@ -35,6 +35,29 @@ def test_struct_layout_matches_header(pkg, tmp_path):
     assert [int(x) for x in out.split()] == expect
 
 
+def test_packed_arguments_match_the_structs(pkg):
+    """The bytes that a call passes are those of the ctypes struct, field by field."""
+    lin, pages = _lin(), graft.submodule("pages")
+    for packed, cls in [(lin._DECODE, pkg._lib.LinDecodeArgs), (lin._PREFILL, pkg._lib.LinPrefillArgs),
+                        (pages._CALLS["fork"], pkg._lib.PagesArgs)]:
+        values = [i + 1 for i in range(len(cls._fields_))]
+        a = cls.from_buffer_copy(packed.pack(*values))
+        got = [getattr(a, f) for f, _ in cls._fields_]
+        got = [ctypes.cast(x, ctypes.c_void_p).value if isinstance(x, ctypes.POINTER(pkg._lib.PagesPool)) else x
+               for x in got]
+        assert got == values
+
+
+def test_values_beyond_a_field_are_refused(pkg):
+    for scale in (1e39, float("inf"), float("nan")):
+        with pytest.raises(pkg.GDNError, match="scale"):
+            _lin()._decode_args(**{**_dec(), "scale": scale})
+        with pytest.raises(pkg.GDNError, match="scale"):
+            _lin()._prefill_args(**{**_pre(), "scale": scale})
+    with pytest.raises(pkg.GDNError, match="pages_copy_launch"):
+        graft.submodule("pages")._CALLS["copy"].pack(0, 0, 1, 0, 0, 1 << 31, *[0] * 7)
+
+
 def decode_args(pkg, **over):
     a = pkg._lib.LinDecodeArgs()
     for i, name in enumerate(("q", "k", "v", "g", "state_in", "o")):
