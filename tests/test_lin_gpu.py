@@ -405,6 +405,67 @@ def test_prefill_packed_long_and_short(pkg):
     assert torch.equal(fin[[4, 6, 7]], pool[[4, 6, 7]])
 
 
+@pytest.mark.parametrize("B", [5, 63, 64, 65])
+def test_prefill_packed_in_any_order(pkg, B):
+    """More CTAs than SMs, so that sequences are taken by length: equal and empty ones, idle rows
+    and unsound offsets among them; each is to the bit what a call of its own gives."""
+    Hv, d, io = 32, 64, torch.bfloat16
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 300, (B,), generator=gen).tolist()
+    lens[1], lens[3], lens[-1] = 0, lens[2], 299
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    T = cu[-1]
+    q, k, v, g = (x.to(DEV) for x in make((1, T), 4, Hv, d, d, io, B))
+    pool = torch.randn(B + 2, Hv, d, d, generator=gen).to(DEV)
+    index = torch.randperm(B + 2, generator=gen)[:B].to(torch.int32)
+    index[2] = -1
+    st = pool.clone()
+    o, _ = pkg.lin_prefill(q, k, v, g, st, index=index.to(DEV), check=True,
+                           cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    want = pool.clone()
+    for n in range(B):
+        if lens[n]:
+            a, b, p = cu[n], cu[n + 1], int(index[n])
+            o1, s1 = pkg.lin_prefill(q[:, a:b], k[:, a:b], v[:, a:b], g[:, a:b], pool[p : p + 1] if p >= 0 else None,
+                                     final_state=torch.empty(1, Hv, d, d, device=DEV))
+            assert torch.equal(o[:, a:b], o1), n
+            if p >= 0:
+                want[p] = s1[0]
+    assert torch.equal(st, want)
+    # the last sequence's end lies behind the rows: it is reported and left out, the others stand
+    cu[-1] = T + 1
+    st2, o2 = pool.clone(), torch.full_like(o, 7.0)
+    with pytest.raises(pkg.GDNError):
+        pkg.lin_prefill(q, k, v, g, st2, index=index.to(DEV), out=o2, check=True,
+                        cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    want[int(index[-1])] = pool[int(index[-1])]
+    assert torch.equal(st2, want)
+    assert torch.equal(o2[:, : cu[-2]], o[:, : cu[-2]]) and bool((o2[:, cu[-2] :] == 7).all())
+
+
+def test_prefill_packed_cut_in_any_order(pkg):
+    """Longest first with one sequence cut in time."""
+    Hv, d, io = 32, 64, torch.bfloat16
+    lens = [70, 300, 1, 8200, 0, 300, 129]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    q, k, v, g = make((1, cu[-1]), Hv, Hv, d, d, io, 41, gmin=-0.05)
+    pool = torch.randn(len(lens), Hv, d, d, generator=torch.Generator().manual_seed(42))
+    st = pool.to(DEV)
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st, final_state=st, scale=0.1, check=True,
+                           cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    o, fin, h = o.cpu(), st.cpu(), [0, 31]
+    for n, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        if a == b:
+            assert torch.equal(fin[n], pool[n])
+            continue
+        ref = steps(q[0, a:b, h], k[0, a:b, h], v[0, a:b, h], g[0, a:b, h], pool[n, h], 0.1)
+        check_prefill(o[0, a:b, h], fin[n, h], ref, io, k[0, a:b, h], v[0, a:b, h])
+
+
 def test_prefill_packed_unsound_offsets_of_long_sequences(pkg):
     """Overlapping long sequences around an unsound one: reported, nothing outside is written."""
     H, d, io, T = 1, 64, torch.bfloat16, 9000
