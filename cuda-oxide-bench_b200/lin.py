@@ -21,6 +21,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
 _DECODE = _lib.Packed(_lib.LinDecodeArgs, "lin_decode_launch")
 _PREFILL = _lib.Packed(_lib.LinPrefillArgs, "lin_prefill_launch")
 _FLOAT_MAX = torch.finfo(torch.float32).max
+_UNCUT = 896  # tokens up to which no prefill is cut in time: no workspace (and 1 us less to ask for it)
 _LOG, _LINEAR = _lib.GATE_LOG, _lib.GATE_LINEAR
 
 
@@ -204,7 +205,7 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
                                       dtype=torch.float32, device=q.device)
     args = (q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale, _status(dev))
     a = _prefill_args(*args)
-    need = _prefill_workspace(a)
+    need = _prefill_workspace(a) if v.shape[1] > _UNCUT else 0
     if need:
         # from the allocator on the current stream, so that calls on other streams
         # and captured graphs have workspaces of their own

@@ -17,6 +17,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from conftest import graft
 from lin_oracle import half_step, steps
 
 pytestmark = pytest.mark.gpu
@@ -485,6 +486,23 @@ def test_prefill_workspace_argument(pkg):
     ws = torch.full((1 << 22,), 255, dtype=torch.uint8, device=DEV)  # whatever it holds before
     got = pkg.lin_prefill(q, k, v, g, workspace=ws, check=True)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_prefill_of_few_tokens_needs_no_workspace(pkg):
+    """What lets a call of few tokens go without asking for the size; a long one needs some."""
+    lin = graft.submodule("lin")
+
+    def need(T, B, H, packed):
+        z = torch.zeros(B, T, H, 64, dtype=torch.bfloat16, device=DEV)
+        cu = torch.zeros(9, dtype=torch.int32, device=DEV) if packed else None
+        fin = torch.empty(8 if packed else B, H, 64, 64, device=DEV)
+        g = torch.zeros(H, device=DEV)
+        return lin._prefill_workspace(lin._prefill_args(z, z, z, g, None, fin, z, cu, None, 1.0))
+
+    for H in (1, 2, 37, 74, 148, 149):
+        for B, packed in ((1, True), (1, False), (2, False), (5, False)):
+            assert need(lin._UNCUT, B, H, packed) == 0
+    assert need(16384, 1, 1, True) > 0 and need(16384, 1, 1, False) > 0
 
 
 def test_prefill_repeats_to_the_bit(pkg):
