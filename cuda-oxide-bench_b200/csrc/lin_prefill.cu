@@ -69,6 +69,7 @@ constexpr int kRanked = 64;
 constexpr float kLowest = -160.f;
 // the factors of e^(G_i - G_j) stay within 2^-kNear .. 2^kNear
 constexpr float kNear = 100.f;
+constexpr float kLeast = 64.f;  // (powers of two)
 // How a chunk's decays are factored, by the range of G (in powers of two):
 //   kNearMid    G spans at most 2 kNear: e^(G_i - M) e^(M - G_j), M its middle
 //   kNearBlock  no gate grows, and each block of 32 tokens spans at most kNear:
@@ -429,12 +430,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float Gi = form == kNearBlock ? bar.ref[st][warp] - __log2f(own) : own;  // (of the other two forms)
       const float f = a.scale * (form == kNearMid ? __frcp_rn(own) : ex2(Gi));
       // SC takes Q as it is.  bf16, and not kFar: so does QS; O then lacks the row's
-      // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: of rows
-      // whose factor is below 2^-kNear, QS takes zeros, and P carries it.)  Else P
-      // carries the row's factor, which its type could not do without, and QS takes
+      // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: a factor
+      // below 2^-kLeast is taken as that; P carries the rest of it, and of the state
+      // before the chunk so little arrives that it makes no difference.)  Else P carries
+      // the row's factor, which its type could not do without, and QS takes
       // Q' = scale e^G Q (bf16) written over Q.
-      const bool by_block = BF16 && form == kNearBlock, live = Gi >= -kNear;
-      const bool plain_q = BF16 && (form == kNearMid || (by_block && __all_sync(0xffffffffu, live)));
+      const bool by_block = BF16 && form == kNearBlock, plain_q = BF16 && form != kFar;
 #pragma unroll 1
       for (int pass = 0; pass < 2; ++pass) {
         if (pass && !(ok = wait(&bar.sc_done, c & 1))) break;
@@ -450,8 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 32; ++i) {
                 uint32_t& w = u[i >> 4][i & 15];
-                w = by_block ? (live ? w : 0u)
-                             : tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
+                w = tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
               }
             }
           tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
@@ -483,10 +483,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
           } else if (by_block) {
             // the block's factor in two steps of at most 2^kNear, or the row's as well
-            const float R = bar.ref[st][b];
-            const float r0 = live ? ex2(-0.5f * R) : a.scale * ex2(Gi - R), r1 = live ? r0 : 1.f;
+            // (its root, twice: the whole may pass the range of a float where d is small)
+            const float r = ex2(0.5f * (Gi - fmaxf(Gi, -kLeast) - bar.ref[st][b]));
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] = d[e] * r0 * r1;
+            for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
           } else if (!BF16) {
             const float r = form == kNearMid ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (BF16 && form == kNearMid) factor = a.scale * __frcp_rn(own);
             if (BF16 && form == kNearBlock) {
               const float Gi = bar.ref[st][quarter] - __log2f(own);
-              if (Gi >= -kNear) factor = a.scale * ex2(Gi);
+              factor = a.scale * ex2(fmaxf(Gi, -kLeast));
             }
             __syncwarp();
           }
