@@ -37,10 +37,12 @@
 // off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
 // state that QS takes, each rounded to bf16 once, give the rest).
 //
-// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 122 us, 403 MB, so
-// 3.3 TB/s or 0.51 of the measured copy): a CTA takes 4700 cycles a chunk.  The
-// tensor pipe is busy for 0.47 of them; shared memory moves about 3900 of the 4700
-// x 128 bytes it could (operands 1280, TMA 1000, the warps' 1600); and instruction
+// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 us, 403 MB, so
+// 3.5 TB/s or 0.54 of the measured copy; 98 us in a burst, before the power limit takes
+// the clock to 1.6 GHz): a CTA takes 5000 cycles a chunk.  The products take 2700 of
+// them, and shared memory moves about 3900 of the 5000 x 128 bytes it could (operands
+// 1280, TMA 1000, the warps' 1600), so that each answer from it, a barrier's too, takes
+// some 250 cycles in the chain Q, SC, P, PV of a chunk.  And instruction
 // fetch: five roles of straight-line code pass through the SM's instruction cache
 // once a chunk, at 0.89 hits.  So loops are kept rolled and call sites single where
 // that is possible; unrolled, the same kernel took 226 us.
@@ -67,15 +69,18 @@ constexpr uint32_t kWaitTries = 1u << 18;
 constexpr int kRanked = 64;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
-// the factors of e^(G_i - G_j) stay within 2^-kNear .. 2^kNear
-constexpr float kNear = 100.f;
-constexpr float kLeast = 64.f;  // (powers of two)
 // How a chunk's decays are factored, by the range of G (in powers of two):
-//   kNearMid    G spans at most 2 kNear: e^(G_i - M) e^(M - G_j), M its middle
+//   kNearMid    G stays within kLeast of its middle M, and M within kLeast of 0:
+//               e^(G_i - M) e^(M - G_j)
 //   kNearBlock  no gate grows, and each block of 32 tokens spans at most kNear:
 //               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
+// In bf16 O is summed without its rows' factors, which are 2^-kLeast at least: fp32 holds
+// outputs of up to 2^47 then, and a row that decay leaves less of the state before the
+// chunk takes 2^-80 of it.
+constexpr float kNear = 100.f;
+constexpr float kLeast = 80.f;
 enum { kNearMid = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
@@ -807,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 16));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 16));
         const float end_of_block = __shfl_sync(0xffffffffu, gv[3], lane | 7);
-        form = hi - lo <= 2.f * kNear && fabsf(hi + lo) <= 2.f * kNear ? kNearMid : near_block ? kNearBlock : kFar;
+        form = hi - lo <= 2.f * kLeast && fabsf(hi + lo) <= 2.f * kLeast ? kNearMid : near_block ? kNearBlock : kFar;
         ref = form == kNearMid ? 0.5f * (lo + hi) : end_of_block;
         if (form != kFar) {
 #pragma unroll

@@ -224,6 +224,24 @@ def test_prefill_gate_ranges(pkg, io, gmin, gmax):
                   k[0], v[0])
 
 
+@pytest.mark.parametrize("gmin", [-0.5, -1.4, -2.5])
+def test_prefill_large_values_under_strong_decay(pkg, gmin):
+    """Sums that leave out the rows' factors stay within fp32's range, and rows of which the state
+    before the chunk has all but vanished take at most 2^-80 of it (v is zero from token 120 on)."""
+    T, d, io = 300, 64, torch.bfloat16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 44, gmin=gmin)
+    v = (v.float() * 2.0 ** 36).to(io)
+    v[:, 120:] = 0
+    S0 = torch.randn(1, 2, d, d)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), check=True)
+    ro, rS, oa, Sa = steps(q[0], k[0], v[0], g[0], S0[0], 1.0)
+    for c in range(0, T, 128):
+        at = steps(q[0, :c], k[0, :c], v[0, :c], g[0, :c], S0[0], 1.0)[3] if c else S0[0].double().abs()
+        rows = slice(c, min(c + 128, T))
+        oa[rows] += 2.0 ** -80 / (half_step(io) + 2 * W) * torch.einsum("td,hde->the", q[0, rows, 0].double().abs(), at)
+    check_prefill(o[0].cpu(), S[0].cpu(), (ro, rS, oa, Sa), io, k[0], v[0])
+
+
 @pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("g_reset", [float("-inf"), -200.0, -1e30])
 def test_prefill_resets(pkg, g_reset, io):
