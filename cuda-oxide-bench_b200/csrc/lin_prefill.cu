@@ -537,18 +537,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           lds64(w + tb * 8, ww[tb]);
           lds64(w + tb * 8 + 4, ww[tb] + 2);
         }
-#pragma unroll 1
+        // all loads first (unrolled 98.2 against 99.5 us; at d = 64 37.9 against 40.7)
+        uint32_t r[2][4][4];
+#pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int dv = quarter * 32 + i * 16;  // of this warp's 16 rows
           const uint32_t block = tile + (dv >> 6) * kTile;
           const int chunk = ((dv & 63) >> 3) + ((lane >> 3) & 1);
-          uint32_t r[4][4], hi[16], lo[16];
 #pragma unroll
           for (int tb = 0; tb < 4; ++tb)
-            tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[tb]);
+            tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[i][tb]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t hi[16], lo[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const uint32_t v = r[e >> 2][e & 3], w_hi = ww[e >> 2][e & 2], w_lo = ww[e >> 2][(e & 2) + 1];
+            const uint32_t v = r[i][e >> 2][e & 3], w_hi = ww[e >> 2][e & 2], w_lo = ww[e >> 2][(e & 2) + 1];
             hi[e] = tc::fma2<BF16>(v, w_hi, tc::mul2<BF16>(v, w_lo));
             lo[e] = tc::fma2<BF16>(v, w_lo, tc::fma2<BF16>(v, w_hi, hi[e] ^ 0x80008000u));
           }
