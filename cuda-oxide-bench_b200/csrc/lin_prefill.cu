@@ -37,15 +37,15 @@
 // off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
 // state that QS takes, each rounded to bf16 once, give the rest).
 //
-// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 us, 403 MB, so
-// 3.5 TB/s or 0.54 of the measured copy; 98 us in a burst, before the power limit takes
-// the clock to 1.6 GHz): a CTA takes 5000 cycles a chunk.  The products take 2700 of
-// them, and shared memory moves about 3900 of the 5000 x 128 bytes it could (operands
-// 1280, TMA 1000, the warps' 1600), so that each answer from it, a barrier's too, takes
-// some 250 cycles in the chain Q, SC, P, PV of a chunk.  And instruction
-// fetch: five roles of straight-line code pass through the SM's instruction cache
-// once a chunk, at 0.89 hits.  So loops are kept rolled and call sites single where
-// that is possible; unrolled, the same kernel took 226 us.
+// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 to 120 us, 403 MB,
+// so 3.4 TB/s or 0.52 of the measured copy; 97 us in a burst, before the power limit
+// takes the clock to 1.6 GHz): a CTA takes 4700 cycles a chunk.  The products take 0.54
+// of them, and shared memory is at work in most: operands 1280 cycles of 128 bytes, TMA
+// 1000, the warps' reads, writes and barriers 2100.  Each answer from it takes some 250
+// cycles then, in the chain Q, SC, P, PV of a chunk.  And instruction fetch: five
+// roles of straight-line code pass through the SM's instruction cache once a chunk, at
+// 0.92 hits.  So loops are kept rolled and call sites single where that is possible;
+// unrolled throughout, the same kernel took 226 us.
 #include <cuda_runtime.h>
 
 #include <atomic>
