@@ -16,6 +16,7 @@
 #include <atomic>
 
 #include "common.cuh"
+#include "page_runs.cuh"
 #include "ptx.cuh"
 
 namespace gdn {
@@ -27,9 +28,8 @@ constexpr int kSmall = 2048;           // pages and entries up to which the copy
 constexpr int64_t kPiece = 32 * 1024;  // bytes of a page that one CTA moves at a time
 // CTAs of a copy: 16 for each SM, of which 4 or so run at a time (16 sources of 2 MB
 // forked into 64 in 2 pools: 65 us with 4, 62 with 8, 58 with 16 and with 64, which
-// each plan for themselves)
+// each plan for themselves; one read for a run of copies of one source: 84 -> 65 us)
 constexpr int kCtasPerSm = 16;
-constexpr int kRun = 8;  // copies of one source that are written with one read (84 -> 65 us there)
 
 enum Op { kCopy, kFork, kCompact };
 
@@ -258,9 +258,9 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   for (int64_t u = blockIdx.x; u < pairs * per; u += gridDim.x) {
     const int64_t i = u / per;
     const int piece = static_cast<int>(u - i * per);
+    int64_t j = run_first(src, dst, pairs, i);
+    if (j < 0) continue;
     const int s = src[i];
-    // entries of one source, up to kRun side by side: the first reads for all of them
-    if (s < 0 || (i % kRun && src[i - 1] == s)) continue;
     int l = 0;
     while (piece >= c.first[l + 1]) ++l;
     const pages_pool_t& pool = c.pool[l];
@@ -273,14 +273,12 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 #pragma unroll
     for (int e = 0; e < static_cast<int>(kPiece / 16 / kCopyThreads); ++e)
       if (e * kCopyThreads + static_cast<int>(threadIdx.x) < n) x[e] = __ldcs(from + e * kCopyThreads + threadIdx.x);
-    for (int64_t j = i;;) {
-      if (dst[j] >= 0) {
-        uint4* to = reinterpret_cast<uint4*>(base + dst[j] * pool.page_stride);
+    for (; j >= 0; j = run_next(src, pairs, j)) {
+      if (dst[j] < 0) continue;
+      uint4* to = reinterpret_cast<uint4*>(base + dst[j] * pool.page_stride);
 #pragma unroll
-        for (int e = 0; e < static_cast<int>(kPiece / 16 / kCopyThreads); ++e)
-          if (e * kCopyThreads + static_cast<int>(threadIdx.x) < n) to[e * kCopyThreads + threadIdx.x] = x[e];
-      }
-      if (++j == pairs || j % kRun == 0 || src[j] != s) break;
+      for (int e = 0; e < static_cast<int>(kPiece / 16 / kCopyThreads); ++e)
+        if (e * kCopyThreads + static_cast<int>(threadIdx.x) < n) to[e * kCopyThreads + threadIdx.x] = x[e];
     }
   }
 }

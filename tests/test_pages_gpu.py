@@ -228,3 +228,25 @@ def test_turn_in_a_graph(pkg):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         assert same(pools, end) and torch.equal(used, flags)
     pkg.check_device_status(torch.device(DEV))
+
+
+def test_sources_just_behind_the_pool(pkg):
+    """Pools that are the front of larger ones: what lies behind is no page, and is neither moved nor needed.
+    Entries of one bad source side by side, in both forms of the plan."""
+    for P, n in ((10, 8), (2500, 2100)):
+        whole = make_pools(P + 4, P)
+        want = copies(whole)
+        pools = [p[:P] for p in whole]
+        src, dst = [P, P, P + 1, 0, 0] + [P] * (n - 5), [1, 2, 3, 4, 4] + list(range(5, n))
+        src[5] = 0  # the one sound entry
+        for p in want:
+            p[5] = p[0]
+        with pytest.raises(pkg.GDNError, match="index"):
+            pkg.pages_copy(pools, i32(src), i32(dst), check=True)
+        assert same(whole, want)
+        used = i32([1, 0, 1] + [1] * (P - 4) + [0])
+        with pytest.raises(pkg.GDNError, match="index"):
+            pkg.pages_fork(pools, used, i32([P, P, 2, 2] + [P + 2] * (n - 4)), check=True)
+        for p in want:
+            p[1], p[P - 1] = p[2], p[2]
+        assert same(whole, want) and used.tolist() == [1] * P
