@@ -37,6 +37,11 @@
 // off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
 // state that QS takes, each rounded to bf16 once, give the rest).
 //
+// A value of V that is not finite belongs to the rows from its own on, but P V would
+// bring it to the earlier ones of its chunk, as 0 x NaN.  V notices it while it makes
+// V'' and puts zero in its place in the tile, and the epilogue writes NaN into its
+// column from its row on.
+//
 // What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 to 120 us, 403 MB,
 // so 3.4 TB/s or 0.52 of the measured copy; 97 us in a burst, before the power limit
 // takes the clock to 1.6 GHz): a CTA takes 4700 cycles a chunk.  The products take 0.54
@@ -102,8 +107,9 @@ struct Layout {
   static constexpr int kO = kS + DK / 64 * kSBlock;
   static constexpr int kGate = kO + BV / 64 * kTile;
   static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
-  static constexpr int kBars = kGate + 2 * kGateStage;
-  static constexpr int kBytes = kBars + 384;
+  static constexpr int kFirst = kGate + 2 * kGateStage;    // per value column, a byte: see Bars::bad
+  static constexpr int kBars = kFirst + 128;
+  static constexpr int kBytes = kBars + 352;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -119,9 +125,12 @@ struct Bars {
   float shift[2];   // e^M (1 unless kNearMid)
   float ref[2][4];  // R_b
   int form[2];      // kNearMid, kNearBlock, kFar
+  // by chunk and V warp: some value of its columns is not finite, and kFirst holds the
+  // first token of which that is so for each of them (kC: none)
+  alignas(8) uint8_t bad[2][4];
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 384, "barriers");
+static_assert(sizeof(Bars) <= 352, "barriers");
 
 struct PrefillParams {
   lin_prefill_args_t a;
@@ -401,6 +410,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.o_stored, 1);
     mbar_init(&bar.zeroed, 4);
     mbar_init(&bar.drain, 1);
+    *reinterpret_cast<uint64_t*>(bar.bad) = 0;  // (warps without columns write none)
     fence_mbar_init();
   }
   if (tid < 4) prefetch_map(tid == 0 ? &map_q : tid == 1 ? &map_k : tid == 2 ? &map_v : &map_o);
@@ -525,9 +535,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp - kWarpV, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const bool has_rows = quarter * 32 < BV;
+    int first = kC;  // the first token of the chunk whose value in column `row` is not finite
     // tokens [64 half, 64 half + 64) of chunk c: both parts
     const auto parts = [&](int c, int half) {
       const int st = c & 1;
+      if (!half) first = kC;
       const uint32_t tile = sb + st * L::kStage + L::kV;
       const uint2* w = reinterpret_cast<const uint2*>(smem + L::kGate + st * L::kGateStage + kC * 4) + half * 32 + (lane & 3);
       if (has_rows) {
@@ -548,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int tb = 0; tb < 4; ++tb)
             tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[i][tb]);
         }
+        uint32_t bad = 0;  // 0 v: zero, or NaN where v is not finite
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t hi[16], lo[16];
@@ -556,22 +569,45 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t v = r[i][e >> 2][e & 3], w_hi = ww[e >> 2][e & 2], w_lo = ww[e >> 2][(e & 2) + 1];
             hi[e] = tc::fma2<BF16>(v, w_hi, tc::mul2<BF16>(v, w_lo));
             lo[e] = tc::fma2<BF16>(v, w_lo, tc::fma2<BF16>(v, w_hi, hi[e] ^ 0x80008000u));
+            if (FULL) bad = tc::fma2<BF16>(v, 0, bad);
           }
           const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + (FULL || half ? kTmV : kTmSC);
           tc::tmem_st_16x128b_x8(to, lo);
           tc::tmem_st_16x128b_x8(to + 32, hi);
         }
         tc::tmem_wait_st();
+        if (FULL && __any_sync(0xffffffffu, bad != 0)) {
+          constexpr uint32_t kExponent = BF16 ? 0x7f80 : 0x7c00;
+          unsigned char* column = smem + st * L::kStage + L::kV + (row >> 6) * kTile + (row & 7) * 2;
+#pragma unroll 1
+          for (int t = half * 64; t < half * 64 + 64; ++t) {
+            uint16_t* x = reinterpret_cast<uint16_t*>(column + tc::sw128_offset(t, (row & 63) >> 3));
+            if ((*x & kExponent) == kExponent) {
+              first = min(first, t);
+              *x = 0;
+            }
+          }
+          tc::fence_proxy_async();
+        }
+        if (FULL && half) {
+          const bool any = __any_sync(0xffffffffu, first < kC);
+          if (any) {  // once every warp has read the marks of the chunk before
+            if (!wait(&bar.o_free, (c & 1) ^ 1)) return false;
+            smem[L::kFirst + row] = static_cast<unsigned char>(first);
+          }
+          if (lane == 0) bar.bad[st][quarter] = any;
+        }
       }
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.v_ready[half]);
+      return true;
     };
     // O of chunk c: a token per thread, times the row's factor, packed into shared memory
     float factor = 1.f;
     const auto output = [&](int c) {
       unsigned char* o = smem + L::kO;
-      if (!wait(&bar.pv_done, c & 1, &bar.o_stored, (c & 1) ^ 1)) return false;
+      if (!wait(&bar.pv_done, c & 1, &bar.o_stored, (c & 1) ^ 1, &bar.v_ready[1], c & 1)) return false;
       tc::fence_after_sync();
 #pragma unroll 1
       for (int b = 0; b < BV / 32; ++b) {
@@ -587,6 +623,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                      tc::pack2<BF16>(factor * y[2], factor * y[3]), tc::pack2<BF16>(factor * y[4], factor * y[5]),
                      tc::pack2<BF16>(factor * y[6], factor * y[7]));
         }
+      }
+      if (*reinterpret_cast<const uint32_t*>(bar.bad[c & 1])) {
+#pragma unroll 1
+        for (int i = 0; i < BV; ++i)
+          if (bar.bad[c & 1][i >> 5] && row >= smem[L::kFirst + i])
+            *reinterpret_cast<uint16_t*>(o + (i >> 6) * kTile + tc::sw128_offset(row, (i & 63) >> 3) + (i & 7) * 2) = 0x7fff;
       }
       tc::fence_before_sync();
       tc::fence_proxy_async();
@@ -638,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int before = FULL ? step - 1 : step - 2;
         if (before >= 0 && !(ok = wait(&bar.v_free[before & 1], (before >> 1) & 1))) break;
         tc::fence_after_sync();
-        parts(c, half);
+        if (!(ok = parts(c, half))) break;
         if (half) {
           if (FULL) {
             const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];

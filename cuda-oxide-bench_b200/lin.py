@@ -187,8 +187,8 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
 
     Few heads and a long T: the time axis is cut, with a workspace from torch's
     allocator (or ``workspace``, at least as large).  Infinities and NaN in a row
-    can reach the rows up to 127 before it in its sequence (they share a chunk),
-    never another sequence.  f16: P = q.k e^(G_i - G_j) scale and e^(G_C - G_j) v
+    reach no earlier row and no other sequence; outputs that a value of v which is
+    not finite belongs to are NaN within its chunk.  f16: P = q.k e^(G_i - G_j) scale and e^(G_C - G_j) v
     have to stay below 65504, which only large values or growing gates pass. bf16:
     under strong decay outputs hold up to 2^47, and a row keeps 2^-80 of the state
     before its chunk where the decay would leave less.

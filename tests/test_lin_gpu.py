@@ -574,3 +574,48 @@ def test_graph_capture_on_another_stream(pkg):
         want_d = pkg.lin_decode(*tok[i], S)
         assert torch.equal(o, want) and torch.equal(od, want_d) and torch.equal(st, S)
     pkg.check_device_status(torch.device(DEV))
+
+
+def check_finite_part(o, S, ref, io, k, v):
+    """What is finite by the definition is so here, and close; the rest is not."""
+    ro, rS, oa, Sa = ref
+    assert torch.equal(torch.isfinite(o), torch.isfinite(ro)) and torch.equal(torch.isfinite(S), torch.isfinite(rS))
+    fo, fS = torch.isfinite(ro), torch.isfinite(rS)
+    zero = torch.zeros((), dtype=torch.float64)
+    k, v = torch.nan_to_num(k.float(), 0, 0, 0), torch.nan_to_num(v.float(), 0, 0, 0)
+    check_prefill(torch.where(fo, o.double(), zero), torch.where(fS, S.double(), zero),
+                  (torch.where(fo, ro, zero), torch.where(fS, rS, zero), torch.where(fo, oa, zero),
+                   torch.where(fS, Sa, zero)), io, k, v)
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 192)])
+@pytest.mark.parametrize("gmin", [-0.2, -2.0, -30.0])
+def test_prefill_values_that_are_not_finite_reach_no_earlier_row(pkg, gmin, dk, dv, io):
+    T, inf, nan = 300, float("inf"), float("nan")
+    q, k, v, g = make((1, T), 1, 2, dk, dv, io, 50, gmin=gmin)
+    S0 = torch.randn(1, 2, dk, dv, generator=torch.Generator().manual_seed(51))
+    q[0, 70, 0, 3] = nan  # its own row alone
+    for t, h, c, x in [(5, 0, 0, inf), (5, 0, 33, nan), (64, 0, 7, -inf), (127, 0, 40, nan), (127, 1, 1, inf), (128, 1, 2, nan),
+                       (200, 1, 63, inf), (130, 1, 62, nan), (299, 0, dv - 1, nan), (3, 1, 62, inf)]:
+        v[0, t, h, c] = x
+    args = [x.to(DEV) for x in (q, k, v, g)]
+    o, S = pkg.lin_prefill(*args, S0.to(DEV), scale=0.1, check=True)
+    check_finite_part(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], S0[0], 0.1), io, k[0], v[0])
+    k[0, 250, 0, 5] = -inf
+    o, S = pkg.lin_prefill(args[0], k.to(DEV), *args[2:], S0.to(DEV), scale=0.1, check=True)
+    check_finite_part(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], S0[0], 0.1), io, k[0], v[0])
+
+
+def test_prefill_padded_batch(pkg):
+    """Sequences of a dense batch that end early, with whatever behind them: their rows are those of the sequence alone."""
+    T, H, d, io = 260, 2, 128, torch.bfloat16
+    q, k, v, g = make((3, T), H, H, d, d, io, 52)
+    lens = [1, 150, 250]
+    for b, n in enumerate(lens):
+        for x in (q, k, v):
+            x[b, n:] = float("nan")
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), check=True)
+    for b, n in enumerate(lens):
+        ref = steps(q[b, :n], k[b, :n], v[b, :n], g[b, :n], torch.zeros(H, d, d), 1.0)
+        check_prefill(o[b, :n].cpu(), ref[1], ref, io, k[b, :n], v[b, :n])
