@@ -853,7 +853,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
           hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
         }
-        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kNear && fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) <= 0.f);
+        // (a NaN, which R_b would bring to the earlier rows of its block, fails this)
+        const bool falls = x[0] <= 0.f && x[1] <= 0.f && x[2] <= 0.f && x[3] <= 0.f;
+        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kNear && falls);
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 8));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 8));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 16));

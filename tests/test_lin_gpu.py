@@ -619,3 +619,14 @@ def test_prefill_padded_batch(pkg):
     for b, n in enumerate(lens):
         ref = steps(q[b, :n], k[b, :n], v[b, :n], g[b, :n], torch.zeros(H, d, d), 1.0)
         check_prefill(o[b, :n].cpu(), ref[1], ref, io, k[b, :n], v[b, :n])
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gmin", [-0.2, -2.0, -30.0])
+@pytest.mark.parametrize("at", [0, 40, 127, 200])
+def test_prefill_nan_gate_reaches_no_earlier_row(pkg, at, gmin, io):
+    T, d = 220, 64
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 53, gmin=gmin)
+    g[0, at, 1] = float("nan")
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), scale=0.1, check=True)
+    check_finite_part(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), 0.1), io, k[0], v[0])
