@@ -75,18 +75,18 @@ constexpr int kRanked = 64;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
 // How a chunk's decays are factored, by the range of G (in powers of two):
-//   kNearMid    G stays within kLeast of its middle M, and M within kLeast of 0:
-//               e^(G_i - M) e^(M - G_j)
-//   kNearBlock  no gate grows, and each block of 32 tokens spans at most kNear:
+//   kNear       G stays between -kLeast and kMost: e^(G_i) e^(-G_j)
+//   kNearBlock  no gate grows, and each block of 32 tokens spans at most kSpan:
 //               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
 // In bf16 O is summed without its rows' factors, which are 2^-kLeast at least: fp32 holds
 // outputs of up to 2^47 then, and a row that decay leaves less of the state before the
-// chunk takes 2^-80 of it.
-constexpr float kNear = 100.f;
-constexpr float kLeast = 80.f;
-enum { kNearMid = 0, kNearBlock = 1, kFar = 2 };
+// chunk takes 2^-80 of it.  The state itself is taken as it is: scaled by a factor in
+// the middle of the range it would leave bf16 below, from 2^-46 on.
+constexpr float kSpan = 100.f;
+constexpr float kLeast = 80.f, kMost = 40.f;
+enum { kNear = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
@@ -102,7 +102,7 @@ struct Layout {
   static constexpr int kV = kK + DK / 64 * kTile;
   static constexpr int kStage = kV + BV / 64 * kTile;
   static constexpr int kQ = 2 * kStage;
-  static constexpr int kS = kQ + DK / 64 * kTile;          // e^M S^T bf16 [BV][DK], 64-wide blocks
+  static constexpr int kS = kQ + DK / 64 * kTile;          // S^T bf16 [BV][DK], 64-wide blocks
   static constexpr int kSBlock = BV * 128;
   static constexpr int kO = kS + DK / 64 * kSBlock;
   static constexpr int kGate = kO + BV / 64 * kTile;
@@ -122,9 +122,8 @@ struct Bars {
   uint64_t v_ready[2], v_free[2], ds_done, ds_free, s_ready;
   uint64_t o_free, o_staged, o_stored, zeroed, drain;
   float gamma[2];
-  float shift[2];   // e^M (1 unless kNearMid)
   float ref[2][4];  // R_b
-  int form[2];      // kNearMid, kNearBlock, kFar
+  int form[2];      // kNear, kNearBlock, kFar
   // by chunk and V warp: some value of its columns is not finite, and kFirst holds the
   // first token of which that is so for each of them (kC: none)
   alignas(8) uint8_t bad[2][4];
@@ -441,9 +440,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(ok = wait(&bar.gfull[st], (c >> 1) & 1, &bar.full[kTileQ][0], c & 1, &bar.qs_done, (c & 1) ^ 1))) break;
       tc::fence_after_sync();
       const int form = bar.form[st];
-      const float own = G[row];  // e^(M - G_i), e^(R - G_i) or G_i
+      const float own = G[row];  // e^(-G_i), e^(R - G_i) or G_i
       const float Gi = form == kNearBlock ? bar.ref[st][warp] - __log2f(own) : own;  // (of the other two forms)
-      const float f = a.scale * (form == kNearMid ? __frcp_rn(own) : ex2(Gi));
+      const float f = a.scale * (form == kNear ? __frcp_rn(own) : ex2(Gi));
       // SC takes Q as it is.  bf16, and not kFar: so does QS; O then lacks the row's
       // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: a factor
       // below 2^-kLeast is taken as that; P carries the rest of it, and of the state
@@ -503,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
           } else if (!BF16) {
-            const float r = form == kNearMid ? f : a.scale * ex2(Gi - bar.ref[st][b]);
+            const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] *= r;
           }
@@ -686,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];
             const int form = bar.form[st];
             factor = 1.f;
-            if (BF16 && form == kNearMid) factor = a.scale * __frcp_rn(own);
+            if (BF16 && form == kNear) factor = a.scale * __frcp_rn(own);
             if (BF16 && form == kNearBlock) {
               const float Gi = bar.ref[st][quarter] - __log2f(own);
               factor = a.scale * ex2(fmaxf(Gi, -kLeast));
@@ -737,15 +736,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!FULL || c + 1 == chunks) continue;
-      if (!(ok = wait(&bar.gfull[(c + 1) & 1], ((c + 1) >> 1) & 1))) break;
-      const float m = bar.shift[(c + 1) & 1];
-      if (has_rows) {  // e^M S^T rounded to bf16, the QS product's operand
+      if (has_rows) {  // S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
           tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7),
-                     tc::pack2<true>(m * S[8 * i], m * S[8 * i + 1]), tc::pack2<true>(m * S[8 * i + 2], m * S[8 * i + 3]),
-                     tc::pack2<true>(m * S[8 * i + 4], m * S[8 * i + 5]), tc::pack2<true>(m * S[8 * i + 6], m * S[8 * i + 7]));
+                     tc::pack2<true>(S[8 * i], S[8 * i + 1]), tc::pack2<true>(S[8 * i + 2], S[8 * i + 3]),
+                     tc::pack2<true>(S[8 * i + 4], S[8 * i + 5]), tc::pack2<true>(S[8 * i + 6], S[8 * i + 7]));
         }
       }
       tc::fence_proxy_async();
@@ -845,8 +842,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         lo = fminf(lo, gv[e]);
         hi = fmaxf(hi, gv[e]);
       }
-      int form = kNearMid;
-      float ref = 0.f;  // M, or R of this lane's block (8 lanes)
+      int form = kNear;
+      float ref = 0.f;  // kNearBlock: R of this lane's block (8 lanes)
       if (FULL) {
 #pragma unroll
         for (int off = 1; off < 8; off <<= 1) {
@@ -855,14 +852,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // (a NaN, which R_b would bring to the earlier rows of its block, fails this)
         const bool falls = x[0] <= 0.f && x[1] <= 0.f && x[2] <= 0.f && x[3] <= 0.f;
-        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kNear && falls);
+        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kSpan && falls);
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 8));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 8));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 16));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 16));
         const float end_of_block = __shfl_sync(0xffffffffu, gv[3], lane | 7);
-        form = hi - lo <= 2.f * kLeast && fabsf(hi + lo) <= 2.f * kLeast ? kNearMid : near_block ? kNearBlock : kFar;
-        ref = form == kNearMid ? 0.5f * (lo + hi) : end_of_block;
+        form = lo >= -kLeast && hi <= kMost ? kNear : near_block ? kNearBlock : kFar;
+        if (form == kNearBlock) ref = end_of_block;
         if (form != kFar) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) gv[e] = ex2(ref - gv[e]);
@@ -879,7 +876,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       *reinterpret_cast<uint4*>(G + kC + lane * 4) = make_uint4(wp[0], wp[1], wp[2], wp[3]);
       if (lane == 0) {
         bar.gamma[st] = ex2(end);
-        bar.shift[st] = form == kNearMid ? ex2(ref) : 1.f;
         bar.form[st] = form;
       }
       if (FULL && (lane & 7) == 7) bar.ref[st][lane >> 3] = ref;

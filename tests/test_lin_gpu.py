@@ -630,3 +630,24 @@ def test_prefill_nan_gate_reaches_no_earlier_row(pkg, at, gmin, io):
     g[0, at, 1] = float("nan")
     o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), scale=0.1, check=True)
     check_finite_part(o[0].cpu(), S[0].cpu(), steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), 0.1), io, k[0], v[0])
+
+
+@pytest.mark.parametrize("gmin", [-0.4, -0.8, -1.6, -3.0])
+def test_prefill_small_states(pkg, gmin):
+    """States and values of 2^-60 keep their relative precision."""
+    T, d, io = 200, 64, torch.bfloat16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 54, gmin=gmin)
+    S0 = torch.randn(1, 2, d, d, generator=torch.Generator().manual_seed(55)) * 2.0 ** -60
+    v = (v.float() * 2.0 ** -60).to(io)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), check=True)
+    ro, rS, oa, Sa = steps(q[0], k[0], v[0], g[0], S0[0], 1.0)
+    u = half_step(io)
+    # below 2^-126, the smallest normal number of bf16 and fp32, nothing is promised
+    tol = u * ro.abs() + (u + 2 * W + 64 * E) * oa + 2.0 ** -126
+    # the rows that decay leaves less than 2^-80 of the state before their chunk take that much
+    for c in range(0, T, 128):
+        at = steps(q[0, :c], k[0, :c], v[0, :c], g[0, :c], S0[0], 1.0)[3] if c else S0[0].double().abs()
+        rows = slice(c, min(c + 128, T))
+        tol[rows] += 2.0 ** -80 * torch.einsum("td,hde->the", q[0, rows, 0].double().abs(), at)
+    assert bool(((o[0].cpu().double() - ro).abs() <= tol).all())
+    assert bool(((S[0].cpu().double() - rS).abs() <= (u * u + 64 * E) * Sa + 2.0 ** -126).all())
