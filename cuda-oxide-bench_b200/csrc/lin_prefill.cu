@@ -54,6 +54,7 @@
 #include <cuda_runtime.h>
 
 #include <atomic>
+#include <cmath>
 #include <type_traits>
 
 #include "common.cuh"
@@ -80,8 +81,8 @@ constexpr float kLowest = -160.f;
 //               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
-// In bf16 O is summed without its rows' factors, which are 2^-kLeast at least: fp32 holds
-// outputs of up to 2^47 then, and a row that decay leaves less of the state before the
+// In bf16 O is summed without its rows' factors, which are 2^-kLeast at least, but with the
+// scale's power of two (2^pow, |pow| <= 32): fp32 holds outputs of up to 2^47 then, and a row that decay leaves less of the state before the
 // chunk takes 2^-80 of it.  The state itself is taken as it is: scaled by a factor in
 // the middle of the range it would leave bf16 below, from 2^-46 on.
 constexpr float kSpan = 100.f;
@@ -140,6 +141,9 @@ struct PrefillParams {
   // contribution; `decay` the pieces' products of gates, [slot][head].
   int piece, pieces, slots;  // pieces: of every sequence, in the dense form
   int ranked;                // packed sequences are taken longest first
+  // scale = rest * 2^pow; bf16 and not kFar: P and the state carry 2^pow, the epilogue
+  // applies the rest
+  float pow, pow2, rest;
   float* slot_state;
   float* decay;
 };
@@ -440,8 +444,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!(ok = wait(&bar.gfull[st], (c >> 1) & 1, &bar.full[kTileQ][0], c & 1, &bar.qs_done, (c & 1) ^ 1))) break;
       tc::fence_after_sync();
       const int form = bar.form[st];
-      const float own = G[row];  // e^(-G_i), e^(R - G_i) or G_i
-      const float Gi = form == kNearBlock ? bar.ref[st][warp] - __log2f(own) : own;  // (of the other two forms)
+      const float own = G[row];  // e^(-G_i) or e^(R - G_i) (bf16: 2^pow of it), or G_i
+      const float Gi = form == kNearBlock ? bar.ref[st][warp] + (BF16 ? p.pow : 0.f) - __log2f(own) : own;  // (not kNear)
       const float f = a.scale * (form == kNear ? __frcp_rn(own) : ex2(Gi));
       // SC takes Q as it is.  bf16, and not kFar: so does QS; O then lacks the row's
       // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: a factor
@@ -687,8 +691,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             factor = 1.f;
             if (BF16 && form == kNear) factor = a.scale * __frcp_rn(own);
             if (BF16 && form == kNearBlock) {
-              const float Gi = bar.ref[st][quarter] - __log2f(own);
-              factor = a.scale * ex2(fmaxf(Gi, -kLeast));
+              const float Gi = bar.ref[st][quarter] + p.pow - __log2f(own);
+              factor = p.rest * ex2(fmaxf(Gi, -kLeast));
             }
             __syncwarp();
           }
@@ -736,13 +740,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       if (!FULL || c + 1 == chunks) continue;
+      float m = 1.f;
+      if (BF16) {
+        if (!(ok = wait(&bar.gfull[(c + 1) & 1], ((c + 1) >> 1) & 1))) break;
+        m = bar.form[(c + 1) & 1] == kFar ? 1.f : p.pow2;
+      }
       if (has_rows) {  // S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
           tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7),
-                     tc::pack2<true>(S[8 * i], S[8 * i + 1]), tc::pack2<true>(S[8 * i + 2], S[8 * i + 3]),
-                     tc::pack2<true>(S[8 * i + 4], S[8 * i + 5]), tc::pack2<true>(S[8 * i + 6], S[8 * i + 7]));
+                     tc::pack2<true>(m * S[8 * i], m * S[8 * i + 1]), tc::pack2<true>(m * S[8 * i + 2], m * S[8 * i + 3]),
+                     tc::pack2<true>(m * S[8 * i + 4], m * S[8 * i + 5]), tc::pack2<true>(m * S[8 * i + 6], m * S[8 * i + 7]));
         }
       }
       tc::fence_proxy_async();
@@ -862,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (form == kNearBlock) ref = end_of_block;
         if (form != kFar) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) gv[e] = ex2(ref - gv[e]);
+          for (int e = 0; e < 4; ++e) gv[e] = ex2(ref - gv[e] + (BF16 ? p.pow : 0.f));
         }
       }
       *reinterpret_cast<float4*>(G + lane * 4) = make_float4(gv[0], gv[1], gv[2], gv[3]);
@@ -1100,6 +1109,10 @@ int launch(const lin_prefill_args_t& a, const Cut& cut, int sms, cudaStream_t st
   static std::atomic<uint64_t> full_done{0}, state_done{0};
   PrefillParams p;
   p.a = a;
+  const int pow = a.scale != 0.f ? ilogbf(a.scale) : 0;
+  p.pow = static_cast<float>(pow < -32 ? -32 : pow > 32 ? 32 : pow);
+  p.pow2 = exp2f(p.pow);
+  p.rest = a.scale / p.pow2;
   p.nvb = a.dv / BV;
   p.piece = cut.piece;
   p.pieces = cut.pieces;

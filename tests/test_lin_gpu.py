@@ -651,3 +651,25 @@ def test_prefill_small_states(pkg, gmin):
         tol[rows] += 2.0 ** -80 * torch.einsum("td,hde->the", q[0, rows, 0].double().abs(), at)
     assert bool(((o[0].cpu().double() - ro).abs() <= tol).all())
     assert bool(((S[0].cpu().double() - rS).abs() <= (u * u + 64 * E) * Sa + 2.0 ** -126).all())
+
+
+@pytest.mark.parametrize("gmin", [-0.5, -1.0, -1.4, -2.5])
+@pytest.mark.parametrize("scale", [2.0 ** -24 * 1.3, -(2.0 ** -9), 2.0 ** 20])
+def test_prefill_large_values_at_any_scale(pkg, scale, gmin):
+    """Outputs of up to 2^43 or so, whatever part of that the scale is."""
+    T, d, io = 300, 64, torch.bfloat16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 56, gmin=gmin)
+    v = (v.float() * 2.0 ** 36 / abs(scale)).to(io)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), scale=scale, check=True)
+    ro, rS, oa, Sa = steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), scale)
+    for c in range(128, T, 128):  # a row takes 2^-80 of the state before its chunk where decay leaves less
+        at = steps(q[0, :c], k[0, :c], v[0, :c], g[0, :c], torch.zeros(2, d, d), scale)[3]
+        rows = slice(c, min(c + 128, T))
+        oa[rows] += abs(scale) * 2.0 ** -80 / (half_step(io) + 2 * W) * torch.einsum("td,hde->the", q[0, rows, 0].double().abs(), at)
+    check_prefill(o[0].cpu(), S[0].cpu(), (ro, rS, oa, Sa), io, k[0], v[0])
+
+
+def test_prefill_scale_of_zero(pkg):
+    q, k, v, g = (x.to(DEV) for x in make((1, 200), 1, 2, 64, 64, torch.bfloat16, 57))
+    o, S = pkg.lin_prefill(q, k, v, g, scale=0.0, check=True)
+    assert bool((o == 0).all()) and torch.equal(S, pkg.lin_prefill(q, k, v, g)[1])
