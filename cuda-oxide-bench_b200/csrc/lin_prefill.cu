@@ -31,10 +31,12 @@
 //
 // V'' = w v, w = e^(G_C - G_j), is split into two parts of the I/O type, hi +
 // lo, because the state is kept to fp32 accuracy: one part would leave half a
-// step of the I/O type of every term (2^-8 in bf16).  So is w, which makes both
-// parts a few packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo =
-// (v w_hi - hi) + v w_lo, the difference being exact.  Against 64 bits the state is
-// off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
+// step of the I/O type of every term (2^-8 in bf16).  In bf16 so is w, which makes
+// both parts a few packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo =
+// (v w_hi - hi) + v w_lo, the difference being exact.  f16 has the range for neither:
+// there w v is formed in fp32 and split times 2^-x, x by the largest of its value
+// column, so that a part is lost only 2^-39 below that; S applies 2^x to dS.  Against
+// 64 bits the state is off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
 // state that QS takes, each rounded to bf16 once, give the rest).
 //
 // A value of V that is not finite belongs to the rows from its own on, but P V would
@@ -109,7 +111,8 @@ struct Layout {
   static constexpr int kGate = kO + BV / 64 * kTile;
   static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
   static constexpr int kFirst = kGate + 2 * kGateStage;    // per value column, a byte: see Bars::bad
-  static constexpr int kBars = kFirst + 128;
+  static constexpr int kShift = kFirst + 128;              // f16: x of V'' per value column, by chunk, a byte
+  static constexpr int kBars = kShift + 2 * 128;
   static constexpr int kBytes = kBars + 352;
   static_assert(kBytes <= 232448, "shared memory");
 };
@@ -406,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
     mbar_init(&bar.pv_done, 1);
-    mbar_init(&bar.ds_done, 1);
+    mbar_init(&bar.ds_done, BF16 ? 1 : 2);
     mbar_init(&bar.s_ready, 8);
     mbar_init(&bar.o_free, 4);
     mbar_init(&bar.o_staged, 4);
@@ -539,39 +542,84 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const bool has_rows = quarter * 32 < BV;
     int first = kC;  // the first token of the chunk whose value in column `row` is not finite
+    // Of this lane's tokens 2 l, 2 l + 1 and 2 l + 8, 2 l + 9 of each 16 of a half, l = lane % 4:
+    // (hi, lo) of w for both tokens of a pair, or (f16) w of each
+    const auto weights = [&](int st, int half, uint32_t (&ww)[4][4]) {
+      const uint2* w = reinterpret_cast<const uint2*>(smem + L::kGate + st * L::kGateStage + kC * 4) + half * 32 + (lane & 3);
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb) {
+        lds64(w + tb * 8, ww[tb]);
+        lds64(w + tb * 8 + 4, ww[tb] + 2);
+      }
+    };
+    // and of columns l / 4 (e even) and l / 4 + 8 of the i-th 16 of this warp, the values
+    const auto values = [&](int st, int half, int i, uint32_t (&r)[4][4]) {
+      const int dv = quarter * 32 + i * 16;
+      const uint32_t block = sb + st * L::kStage + L::kV + (dv >> 6) * kTile;
+      const int chunk = ((dv & 63) >> 3) + ((lane >> 3) & 1);
+#pragma unroll
+      for (int tb = 0; tb < 4; ++tb)
+        tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[tb]);
+    };
+    float shrink[2][2] = {};  // f16: 2^-x of those columns
+    // x: the largest |w v| of a column times 2^-x lies in [2^13, 2^14)
+    const auto find_shifts = [&](int st) {
+      float most[2][2] = {};
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        uint32_t ww[4][4], r[4][4];
+        weights(st, half, ww);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          values(st, half, i, r);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t v = r[e >> 2][e & 3];
+            float& m = most[i][e & 1];
+            m = fmaxf(m, fabsf(__uint_as_float(ww[e >> 2][e & 2]) * tc::unpack_lo<BF16>(v)));
+            m = fmaxf(m, fabsf(__uint_as_float(ww[e >> 2][(e & 2) + 1]) * tc::unpack_hi<BF16>(v)));
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float m = most[i >> 1][i & 1];
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // (below 2^-100 columns keep less; above, 2^115 for infinities)
+        const int x = max(static_cast<int>(__float_as_uint(m) >> 23) - 127 - 13, -113);
+        shrink[i >> 1][i & 1] = __uint_as_float(static_cast<uint32_t>(127 - x) << 23);
+        if ((lane & 3) == 0)
+          smem[L::kShift + st * 128 + quarter * 32 + i * 8 + (lane >> 2)] = static_cast<unsigned char>(x);
+      }
+    };
     // tokens [64 half, 64 half + 64) of chunk c: both parts
     const auto parts = [&](int c, int half) {
       const int st = c & 1;
       if (!half) first = kC;
-      const uint32_t tile = sb + st * L::kStage + L::kV;
-      const uint2* w = reinterpret_cast<const uint2*>(smem + L::kGate + st * L::kGateStage + kC * 4) + half * 32 + (lane & 3);
       if (has_rows) {
-        uint32_t ww[4][4];  // (hi, lo) of tokens 2 l, 2 l + 1 and 2 l + 8, 2 l + 9 of each 16, l = lane % 4
-#pragma unroll
-        for (int tb = 0; tb < 4; ++tb) {
-          lds64(w + tb * 8, ww[tb]);
-          lds64(w + tb * 8 + 4, ww[tb] + 2);
-        }
+        if (!BF16 && !half) find_shifts(st);
+        uint32_t ww[4][4], r[2][4][4];
+        weights(st, half, ww);
         // all loads first (unrolled 98.2 against 99.5 us; at d = 64 37.9 against 40.7)
-        uint32_t r[2][4][4];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int dv = quarter * 32 + i * 16;  // of this warp's 16 rows
-          const uint32_t block = tile + (dv >> 6) * kTile;
-          const int chunk = ((dv & 63) >> 3) + ((lane >> 3) & 1);
-#pragma unroll
-          for (int tb = 0; tb < 4; ++tb)
-            tc::ldsm_x4_trans(block + tc::sw128_offset(half * 64 + tb * 16 + (lane >> 4) * 8 + (lane & 7), chunk), r[i][tb]);
-        }
+        values(st, half, 0, r[0]);
+        values(st, half, 1, r[1]);
         uint32_t bad = 0;  // 0 v: zero, or NaN where v is not finite
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            const uint32_t v = r[i][e >> 2][e & 3], w_hi = ww[e >> 2][e & 2], w_lo = ww[e >> 2][(e & 2) + 1];
-            hi[e] = tc::fma2<BF16>(v, w_hi, tc::mul2<BF16>(v, w_lo));
-            lo[e] = tc::fma2<BF16>(v, w_lo, tc::fma2<BF16>(v, w_hi, hi[e] ^ 0x80008000u));
+            const uint32_t v = r[i][e >> 2][e & 3], w0 = ww[e >> 2][e & 2], w1 = ww[e >> 2][(e & 2) + 1];
+            if constexpr (BF16) {
+              hi[e] = tc::fma2<BF16>(v, w0, tc::mul2<BF16>(v, w1));
+              lo[e] = tc::fma2<BF16>(v, w1, tc::fma2<BF16>(v, w0, hi[e] ^ 0x80008000u));
+            } else {
+              const float x = __uint_as_float(w0) * tc::unpack_lo<BF16>(v) * shrink[i][e & 1];
+              const float y = __uint_as_float(w1) * tc::unpack_hi<BF16>(v) * shrink[i][e & 1];
+              hi[e] = tc::pack2<BF16>(x, y);
+              lo[e] = tc::pack2<BF16>(x - tc::unpack_lo<BF16>(hi[e]), y - tc::unpack_hi<BF16>(hi[e]));
+            }
             if (FULL) bad = tc::fma2<BF16>(v, 0, bad);
           }
           const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + (FULL || half ? kTmV : kTmSC);
@@ -723,13 +771,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         const float gamma = bar.gamma[st];
         if (has_rows) {
+          const int x = BF16 ? 0 : static_cast<signed char>(smem[L::kShift + st * 128 + row]);
+          const float grow = __uint_as_float(static_cast<uint32_t>(127 + x) << 23);
 #pragma unroll
           for (int b = 0; b < kN / 16; ++b) {
             float d[16];
             tc::tmem_ld16(tmem + lanes + kTmDS + half * kN + b * 16, d);
             tc::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], d[e]);
+            for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], BF16 ? d[e] : grow * d[e]);
           }
         }
         tc::fence_before_sync();
@@ -875,12 +925,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       *reinterpret_cast<float4*>(G + lane * 4) = make_float4(gv[0], gv[1], gv[2], gv[3]);
-      // the weights of two tokens in two parts of the I/O type: (hi, hi), (lo, lo)
       uint32_t wp[4];
 #pragma unroll
       for (int e = 0; e < 4; e += 2) {
-        wp[e] = tc::pack2<BF16>(wv[e], wv[e + 1]);
-        wp[e + 1] = tc::pack2<BF16>(wv[e] - tc::unpack_lo<BF16>(wp[e]), wv[e + 1] - tc::unpack_hi<BF16>(wp[e]));
+        if (BF16) {  // the weights of two tokens in two parts: (hi, hi), (lo, lo)
+          wp[e] = tc::pack2<BF16>(wv[e], wv[e + 1]);
+          wp[e + 1] = tc::pack2<BF16>(wv[e] - tc::unpack_lo<BF16>(wp[e]), wv[e + 1] - tc::unpack_hi<BF16>(wp[e]));
+        } else {
+          wp[e] = __float_as_uint(wv[e]);
+          wp[e + 1] = __float_as_uint(wv[e + 1]);
+        }
       }
       *reinterpret_cast<uint4*>(G + kC + lane * 4) = make_uint4(wp[0], wp[1], wp[2], wp[3]);
       if (lane == 0) {
@@ -956,6 +1010,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       add_ds(1);
       tc::commit(&bar.v_free[1]);
       tc::commit(&bar.ds_done);
+      if (!BF16) mbar_arrive(&bar.ds_done);  // (hands V's shifts on to S)
       tc::commit(&bar.empty[kTileK][st]);
 
       if constexpr (FULL) {

@@ -673,3 +673,33 @@ def test_prefill_scale_of_zero(pkg):
     q, k, v, g = (x.to(DEV) for x in make((1, 200), 1, 2, 64, 64, torch.bfloat16, 57))
     o, S = pkg.lin_prefill(q, k, v, g, scale=0.0, check=True)
     assert bool((o == 0).all()) and torch.equal(S, pkg.lin_prefill(q, k, v, g)[1])
+
+
+@pytest.mark.parametrize("early,late,gmin", [(1000.0, 1e-3, -0.25), (6e4, 1e-4, -0.2), (1.0, 0.0, -0.4), (2.0 ** -14, 2.0 ** -20, -0.1),
+                                             (2.0 ** -24, 2.0 ** -24, 0.0), (1.0, 1.0, -0.2), (6e4, 6e4, 0.0)])
+def test_prefill_f16_state_of_uneven_values(pkg, early, late, gmin):
+    """Large values that have decayed by the chunk's end beside small ones, and values near f16's ends.  What is
+    left of the two parts of a term is u^2 of it, and 2^-39 of its column's largest in the chunk, 128 times."""
+    T, dk, dv, io = 256, 64, 128, torch.float16
+    q, k, v, g = make((1, T), 1, 2, dk, dv, io, 58, gmin=gmin)
+    size = torch.where(torch.arange(T) % 128 < 20, early, late)[:, None, None]
+    v = (torch.rand(T, 2, dv, generator=torch.Generator().manual_seed(59)) * 2 - 1) * size
+    v[:, :, 1::2] *= 2.0 ** -8  # columns next to one another differ too
+    v = v.to(io)[None]
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), scale=2.0 ** -7, check=True)
+    _, rS, _, Sa = steps(q[0], k[0], v[0], g[0], torch.zeros(2, dk, dv), 2.0 ** -7)
+    u = half_step(io)
+    tol = (u * u + 64 * E) * Sa + 2.0 ** -32 * Sa.amax(1, keepdim=True)
+    assert bool(((S[0].cpu().double() - rS).abs() <= tol).all()), float(((S[0].cpu().double() - rS).abs() / tol).max())
+
+
+def test_prefill_f16_growing_gates_keep_the_state(pkg):
+    """Weights e^(G_C - G_j) far beyond f16's range."""
+    T, d, io = 200, 64, torch.float16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 60, gmin=0.5)
+    v = (v.float() * 2.0 ** -10).to(io)
+    _, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), check=True)
+    _, rS, _, Sa = steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), 1.0)
+    u = half_step(io)
+    assert float(rS.abs().max()) > 2.0 ** 40
+    assert bool(((S[0].cpu().double() - rS).abs() <= (u * u + 64 * E) * Sa + 2.0 ** -32 * Sa.amax(1, keepdim=True)).all())
