@@ -25,7 +25,9 @@
 //   D1  dS^T += V''^T K            of the others; then S reads dS and rewrites S^T
 //   PV  O    += P V                then V applies the rows' factors and stages O
 // D0 and D1 lie between the others so that the tensor cores have work while R and
-// V prepare the next operand.  All five take A from TMEM: a product with both
+// V prepare the next operand.  With f16 I/O QS, which R makes ready last, comes after
+// D1, and is three products: queries and state each in two parts of bf16, which has
+// the range for them, 2^-17 off.  All five take A from TMEM: a product with both
 // operands in shared memory reads it at its full rate, and other warps' reads then
 // take five times as long (4 ldmatrix.x4: 726 cycles against 141).
 //
@@ -93,21 +95,25 @@ enum { kNear = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
+constexpr uint32_t kTmQLow = 64;  // f16: the lower part of Q' [DK / 2]
 constexpr uint32_t kTmQ = 128;    // Q, or Q' in bf16 [DK / 2]
 constexpr uint32_t kTmV = 192;    // V'': lo [32], hi [32] of 64 tokens
 constexpr uint32_t kTmO = 256;    // O fp32 [BV]
 constexpr uint32_t kTmDS = 384;   // dS^T fp32 [DK]
 
-template <int DK, int BV>
+template <int DK, int BV, bool BF16, bool FULL>
 struct Layout {
-  // K and V in two stages; Q, which R takes into TMEM at once, in one
+  // K and V in two stages; Q, which R takes into TMEM, in one, and K too where the two
+  // parts of S^T need its place
+  static constexpr int kKStages = !BF16 && FULL && DK == 128 && BV == 128 ? 1 : 2;
+  static constexpr int kKTile = DK / 64 * kTile, kVTile = BV / 64 * kTile;
   static constexpr int kK = 0;
-  static constexpr int kV = kK + DK / 64 * kTile;
-  static constexpr int kStage = kV + BV / 64 * kTile;
-  static constexpr int kQ = 2 * kStage;
-  static constexpr int kS = kQ + DK / 64 * kTile;          // S^T bf16 [BV][DK], 64-wide blocks
+  static constexpr int kV = kKStages * kKTile;
+  static constexpr int kQ = kV + 2 * kVTile;
+  static constexpr int kS = kQ + DK / 64 * kTile;          // S^T bf16 [BV][DK], 64-wide blocks; f16: high, low part
   static constexpr int kSBlock = BV * 128;
-  static constexpr int kO = kS + DK / 64 * kSBlock;
+  static constexpr int kSPart = DK / 64 * kSBlock;
+  static constexpr int kO = kS + (BF16 || !FULL ? 1 : 2) * kSPart;
   static constexpr int kGate = kO + BV / 64 * kTile;
   static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
   static constexpr int kFirst = kGate + 2 * kGateStage;    // per value column, a byte: see Bars::bad
@@ -383,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     lin_prefill_kernel(const __grid_constant__ PrefillParams p, const __grid_constant__ CUtensorMap map_q,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                        const __grid_constant__ CUtensorMap map_o) {
-  using L = Layout<DK, BV>;
-  constexpr bool BF16 = sizeof(IO) == 2 && std::is_same<IO, __nv_bfloat16>::value;
+  constexpr bool BF16 = std::is_same<IO, __nv_bfloat16>::value;
+  using L = Layout<DK, BV, BF16, FULL>;
   extern __shared__ __align__(1024) unsigned char smem[];
   Bars& bar = *reinterpret_cast<Bars*>(smem + L::kBars);
   const lin_prefill_args_t& a = p.a;
@@ -454,39 +460,51 @@ __global__ void __launch_bounds__(kThreads, 1)
       // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: a factor
       // below 2^-kLeast is taken as that; P carries the rest of it, and of the state
       // before the chunk so little arrives that it makes no difference.)  Else P carries
-      // the row's factor, which its type could not do without, and QS takes
-      // Q' = scale e^G Q (bf16) written over Q.
+      // the row's factor, which its type could not do without, and QS takes Q' = scale
+      // e^G Q written over Q: in bf16, whose range it needs, and with f16 I/O in two
+      // parts of it, the lower one over the scores that P leaves free.
       const bool by_block = BF16 && form == kNearBlock, plain_q = BF16 && form != kFar;
+      const auto queries = [&](bool scaled) {
 #pragma unroll 1
-      for (int pass = 0; pass < 2; ++pass) {
+        for (int b = 0; b < DK / 64; ++b) {
+          uint32_t u[2][16];
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            lds128(smem + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
+          if (scaled) {
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+              uint32_t lo[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                uint32_t& w = u[h2][i];
+                const float x = f * tc::unpack_lo<BF16>(w), y = f * tc::unpack_hi<BF16>(w);
+                w = tc::pack2<true>(x, y);
+                if (!BF16) lo[i] = tc::pack2<true>(x - tc::unpack_lo<true>(w), y - tc::unpack_hi<true>(w));
+              }
+              if (!BF16) tc::tmem_st16(tmem + lanes + kTmQLow + b * 32 + h2 * 16, lo);
+            }
+          }
+          tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
+          tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
+        }
+      };
+#pragma unroll 1
+      for (int pass = 0; pass < (BF16 ? 2 : 1); ++pass) {
         if (pass && !(ok = wait(&bar.sc_done, c & 1))) break;
         tc::fence_after_sync();
         if (!pass || !plain_q) {
-#pragma unroll 1
-          for (int b = 0; b < DK / 64; ++b) {
-            uint32_t u[2][16];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              lds128(smem + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
-            if (pass) {
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                uint32_t& w = u[i >> 4][i & 15];
-                w = tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
-              }
-            }
-          tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
-            tc::tmem_st16(tmem + lanes + kTmQ + b * 32 + 16, u[1]);
-          }
+          queries(pass);
           tc::tmem_wait_st();
           tc::fence_before_sync();
           __syncwarp();
         }
         if (lane == 0) {
           mbar_arrive(pass ? &bar.q2_ready : &bar.q_ready);
-          if (pass != plain_q) mbar_arrive(&bar.empty[kTileQ][0]);  // read for the last time
+          if (BF16 && pass != plain_q) mbar_arrive(&bar.empty[kTileQ][0]);  // read for the last time
         }
       }
+      if (!BF16 && (ok = wait(&bar.sc_done, c & 1))) tc::fence_after_sync();
       if (!ok) break;
       // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
 #pragma unroll 1
@@ -528,10 +546,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
       }
+      if (!BF16) queries(true);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) {
+        if (!BF16) mbar_arrive(&bar.empty[kTileQ][0]);
         mbar_arrive(&bar.p_ready);
         mbar_arrive(&bar.gempty[st]);
       }
@@ -555,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // and of columns l / 4 (e even) and l / 4 + 8 of the i-th 16 of this warp, the values
     const auto values = [&](int st, int half, int i, uint32_t (&r)[4][4]) {
       const int dv = quarter * 32 + i * 16;
-      const uint32_t block = sb + st * L::kStage + L::kV + (dv >> 6) * kTile;
+      const uint32_t block = sb + L::kV + st * L::kVTile + (dv >> 6) * kTile;
       const int chunk = ((dv & 63) >> 3) + ((lane >> 3) & 1);
 #pragma unroll
       for (int tb = 0; tb < 4; ++tb)
@@ -629,7 +649,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::tmem_wait_st();
         if (FULL && __any_sync(0xffffffffu, bad != 0)) {
           constexpr uint32_t kExponent = BF16 ? 0x7f80 : 0x7c00;
-          unsigned char* column = smem + st * L::kStage + L::kV + (row >> 6) * kTile + (row & 7) * 2;
+          unsigned char* column = smem + L::kV + st * L::kVTile + (row >> 6) * kTile + (row & 7) * 2;
 #pragma unroll 1
           for (int t = half * 64; t < half * 64 + 64; ++t) {
             uint16_t* x = reinterpret_cast<uint16_t*>(column + tc::sw128_offset(t, (row & 63) >> 3));
@@ -715,12 +735,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (rows < kC) {
             // rows of the next sequence, or outside: zero, whatever they hold, since
             // 0 x NaN would reach the sums over the chunk's tokens
-            if (!(ok = wait(&bar.full[kTileK][st], ph))) break;
-            unsigned char* stage = smem + st * L::kStage;
+            const int kst = c & (L::kKStages - 1);
+            if (!(ok = wait(&bar.full[kTileK][kst], (c / L::kKStages) & 1))) break;
             for (int r = rows + quarter; r < kC; r += 4)
-              for (int i = lane; i < (DK + BV) / 8; i += 32)
-                *reinterpret_cast<uint4*>(stage + L::kK + (i >> 3) * kTile + tc::sw128_offset(r, i & 7)) =
-                    make_uint4(0, 0, 0, 0);
+              for (int i = lane; i < (DK + BV) / 8; i += 32) {
+                const int b = i >> 3;
+                unsigned char* to = smem + (b < DK / 64 ? L::kK + kst * L::kKTile + b * kTile
+                                                        : L::kV + st * L::kVTile + (b - DK / 64) * kTile);
+                *reinterpret_cast<uint4*>(to + tc::sw128_offset(r, i & 7)) = make_uint4(0, 0, 0, 0);
+              }
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&bar.zeroed);
@@ -794,11 +817,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (BF16) {
         if (!(ok = wait(&bar.gfull[(c + 1) & 1], ((c + 1) >> 1) & 1))) break;
         m = bar.form[(c + 1) & 1] == kFar ? 1.f : p.pow2;
+      } else if (c >= 0 && !(ok = wait(&bar.qs_done, c & 1))) {
+        break;  // (in bf16 ds_done comes behind it)
       }
       if (has_rows) {  // S^T rounded to bf16, the QS product's operand
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
+          if (!BF16) {  // the lower part; the upper one as in bf16
+            uint32_t lo[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t hi = tc::pack2<true>(S[8 * i + 2 * e], S[8 * i + 2 * e + 1]);
+              lo[e] = tc::pack2<true>(S[8 * i + 2 * e] - tc::unpack_lo<true>(hi), S[8 * i + 2 * e + 1] - tc::unpack_hi<true>(hi));
+            }
+            tc::sts128(sb + L::kS + L::kSPart + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7), lo[0], lo[1], lo[2], lo[3]);
+          }
           tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7),
                      tc::pack2<true>(m * S[8 * i], m * S[8 * i + 1]), tc::pack2<true>(m * S[8 * i + 2], m * S[8 * i + 3]),
                      tc::pack2<true>(m * S[8 * i + 4], m * S[8 * i + 5]), tc::pack2<true>(m * S[8 * i + 6], m * S[8 * i + 7]));
@@ -815,20 +849,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kWarpTma) {
     if (tc::elect_one()) {
-      // In the order in which the tiles come free (the second chunk's Q waits for the
-      // first's); a tile's barrier is armed only then, its last load being complete.
+      // In the order in which the tiles come free (bf16: the second chunk's Q waits for the
+      // first's; f16: R reads Q to its end); a tile's barrier is armed only then, its last
+      // load being complete.
+      constexpr int kStages[3] = {1, L::kKStages, 2};
       int armed[3] = {0, 0, 0};
       for (int c = 0; c < chunks && ok; ++c) {
         const int t = seq.start + c * kC;
 #pragma unroll 1
         for (int i = 0; i < 3 && ok; ++i) {
-          const int tile = c == 1 ? (i + 1) % 3 : i;
+          const int tile = !BF16 ? 2 - i : c == 1 ? (i + 1) % 3 : i;
           if (!FULL && tile == kTileQ) continue;
-          const int stages = tile == kTileQ ? 1 : 2, st = c & (stages - 1);
+          const int stages = tile == kTileQ ? 1 : tile == kTileK ? L::kKStages : 2, st = c & (stages - 1);
           const int blocks = tile == kTileV ? BV / 64 : DK / 64;
           const int x = tile == kTileV ? vb * BV : 0, head = tile == kTileV ? h : hq;
           const CUtensorMap* map = tile == kTileQ ? &map_q : tile == kTileK ? &map_k : &map_v;
-          unsigned char* to = smem + (tile == kTileQ ? L::kQ : st * L::kStage + (tile == kTileK ? L::kK : L::kV));
+          unsigned char* to = smem + (tile == kTileQ ? L::kQ : tile == kTileK ? L::kK + st * L::kKTile : L::kV + st * L::kVTile);
           if (c >= stages && !(ok = wait1(&bar.empty[tile][st], (c / stages - 1) & 1))) break;
           mbar_arrive_expect_tx(&bar.full[tile][st], blocks * kTile);
           for (int b = 0; b < blocks; ++b) tc::tma_load_4d(to + b * kTile, map, x + b * 64, head, t, batch, &bar.full[tile][st]);
@@ -838,7 +874,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // no copy may be in flight when the shared memory is released
 #pragma unroll
       for (int tile = 0; tile < 3; ++tile) {
-        const int stages = tile == kTileQ ? 1 : 2;
+        const int stages = kStages[tile];
         for (int j = max(0, armed[tile] - stages); j < armed[tile]; ++j)
           if (!wait1(&bar.full[tile][j & (stages - 1)], (j / stages) & 1)) ok = false;
       }
@@ -966,11 +1002,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t kIdPV = tc::idesc_f16(128, BV, false, true, BF16);
 #pragma unroll 1
     for (int c = 0; c < chunks; ++c) {
-      const int st = c & 1;
+      const int st = c & 1, kst = c & (L::kKStages - 1);
+      const uint32_t kph = (c / L::kKStages) & 1;
       // step s of an operand lies a constant number of 16-byte units after step 0
-      const uint32_t stage = sb + st * L::kStage;
-      const uint64_t k = tc::kmajor_desc(stage + L::kK, kTile, 0);
-      const uint64_t kt = tc::mnmajor_desc(stage + L::kK, kTile, 0), v = tc::mnmajor_desc(stage + L::kV, kTile, 0);
+      const uint32_t k_at = sb + L::kK + kst * L::kKTile;
+      const uint64_t k = tc::kmajor_desc(k_at, kTile, 0);
+      const uint64_t kt = tc::mnmajor_desc(k_at, kTile, 0), v = tc::mnmajor_desc(sb + L::kV + st * L::kVTile, kTile, 0);
       const uint64_t sT = tc::kmajor_desc(sb + L::kS, L::kSBlock, 0);
       const auto along = [](int s, int block) { return static_cast<uint64_t>(((s >> 2) * block + (s & 3) * 32) >> 4); };
       const auto add_ds = [&](int half) {  // 64 tokens: the small parts, then the large ones
@@ -979,7 +1016,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc::mma_tmem_a(kTmDS, (FULL || half ? kTmV : kTmSC) + s * 8, kt + half * 512 + (s & 3) * 128, kIdDS, half || s > 0);
       };
       if constexpr (FULL) {
-        ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1, &bar.q_ready, c & 1, &bar.pv_done, (c & 1) ^ 1);
+        ok = wait1(&bar.full[kTileK][kst], kph, &bar.q_ready, c & 1, &bar.pv_done, (c & 1) ^ 1);
         if (!ok) break;
         tc::fence_after_sync();
 #pragma unroll
@@ -988,13 +1025,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::commit(&bar.sc_done);
       }
 
-      ok = wait1(&bar.full[kTileK][st], (c >> 1) & 1, &bar.v_ready[0], c & 1, &bar.ds_free, (c & 1) ^ 1);
+      ok = wait1(&bar.full[kTileK][kst], kph, &bar.v_ready[0], c & 1, &bar.ds_free, (c & 1) ^ 1);
       if (!ok) break;
       tc::fence_after_sync();
       add_ds(0);
       tc::commit(&bar.v_free[0]);
 
-      if constexpr (FULL) {
+      if constexpr (FULL && BF16) {
         ok = wait1(&bar.q2_ready, c & 1, &bar.s_ready, c & 1, &bar.o_free, (c & 1) ^ 1);
         if (!ok) break;
         tc::fence_after_sync();
@@ -1011,12 +1048,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&bar.v_free[1]);
       tc::commit(&bar.ds_done);
       if (!BF16) mbar_arrive(&bar.ds_done);  // (hands V's shifts on to S)
-      tc::commit(&bar.empty[kTileK][st]);
+      tc::commit(&bar.empty[kTileK][kst]);
 
       if constexpr (FULL) {
-        ok = wait1(&bar.p_ready, c & 1);
+        if (BF16) ok = wait1(&bar.p_ready, c & 1);
+        else ok = wait1(&bar.p_ready, c & 1, &bar.s_ready, c & 1, &bar.o_free, (c & 1) ^ 1);
         if (!ok) break;
         tc::fence_after_sync();
+        if constexpr (!BF16) {  // lower part of Q', lower part of S^T, the upper ones
+#pragma unroll
+          for (int part = 0; part < 3; ++part)
+#pragma unroll
+            for (int s = 0; s < DK / 16; ++s)
+              tc::mma_tmem_a(kTmO, (part ? kTmQ : kTmQLow) + s * 8, sT + along(s, L::kSBlock) + (part == 1 ? L::kSPart >> 4 : 0),
+                             kIdQS, part || s > 0);
+          tc::commit(&bar.qs_done);
+        }
 #pragma unroll
         for (int s = 0; s < kC / 16; ++s)
           tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
@@ -1160,7 +1207,8 @@ Cut choose_cut(const lin_prefill_args_t& a, int sms) {
 template <int DK, int BV, typename IO>
 int launch(const lin_prefill_args_t& a, const Cut& cut, int sms, cudaStream_t stream) {
   constexpr bool bf = std::is_same<IO, __nv_bfloat16>::value;
-  using L = Layout<DK, BV>;
+  using L = Layout<DK, BV, bf, true>;
+  using LState = Layout<DK, BV, bf, false>;
   static std::atomic<uint64_t> full_done{0}, state_done{0};
   PrefillParams p;
   p.a = a;
@@ -1186,8 +1234,8 @@ int launch(const lin_prefill_args_t& a, const Cut& cut, int sms, cudaStream_t st
   const unsigned rows = static_cast<unsigned>(a.Hv * p.nvb), slots = static_cast<unsigned>(cut.slots);
   if (slots) {
     const int64_t page = static_cast<int64_t>(a.Hv) * a.dk * a.dv;
-    if ((rc = ensure_smem_attr(lin_prefill_kernel<DK, BV, IO, false>, L::kBytes, state_done)) ||
-        (rc = launch_pdl(lin_prefill_kernel<DK, BV, IO, false>, dim3(rows, slots), kThreads, L::kBytes, stream, p, mq, mk, mv, mo)) ||
+    if ((rc = ensure_smem_attr(lin_prefill_kernel<DK, BV, IO, false>, LState::kBytes, state_done)) ||
+        (rc = launch_pdl(lin_prefill_kernel<DK, BV, IO, false>, dim3(rows, slots), kThreads, LState::kBytes, stream, p, mq, mk, mv, mo)) ||
         (rc = launch_pdl(lin_scan_kernel, dim3(static_cast<unsigned>((page + 1023) / 1024), static_cast<unsigned>(a.B)), 256, 0,
                          stream, p)))
       return rc;

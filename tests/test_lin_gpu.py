@@ -703,3 +703,45 @@ def test_prefill_f16_growing_gates_keep_the_state(pkg):
     u = half_step(io)
     assert float(rS.abs().max()) > 2.0 ** 40
     assert bool(((S[0].cpu().double() - rS).abs() <= (u * u + 64 * E) * Sa + 2.0 ** -32 * Sa.amax(1, keepdim=True)).all())
+
+
+def check_f16_rows(o, ref, v):
+    """f16 I/O: the output's rounding and that of P (u each of its terms; numbers below 2^-14 by at most 2^-25),
+    queries and states in two parts of bf16 (each 2^-18, the product of the lower parts as much)."""
+    ro, _, oa, _ = ref
+    u = half_step(torch.float16)
+    tol = u * ro.abs() + 2.0 ** -25 + (u + 2.0 ** -16 + 64 * E) * oa + 2.0 ** -25 * 128 * v.double().abs().amax()
+    assert bool(((o.double() - ro).abs() <= tol).all()), float(((o.double() - ro).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dk,dv", [(64, 64), (64, 128), (128, 64), (128, 128), (128, 192)])
+@pytest.mark.parametrize("T,gmin", [(1, -0.2), (130, 0.0), (257, -0.05), (400, -0.5), (400, -2.0)])
+def test_prefill_f16_outputs(pkg, T, gmin, dk, dv):
+    """Queries and states are not held in bf16 alone where the I/O is f16."""
+    io = torch.float16
+    q, k, v, g = make((1, T), 1, 2, dk, dv, io, 61, gmin=gmin)
+    S0 = torch.randn(1, 2, dk, dv, generator=torch.Generator().manual_seed(62)) * 30
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=0.05, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], S0[0], 0.05)
+    check_f16_rows(o[0].cpu(), ref, v)
+    check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0], v[0])
+
+
+def test_prefill_f16_states_beyond_its_range(pkg):
+    """A state that f16 does not hold, queries that make its outputs small."""
+    T, d, io = 200, 128, torch.float16
+    q, k, v, g = make((1, T), 1, 1, d, d, io, 63, gmin=-0.01)
+    S0 = torch.randn(1, 1, d, d, generator=torch.Generator().manual_seed(64)) * 1e7
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=2.0 ** -15, check=True)
+    check_f16_rows(o[0].cpu(), steps(q[0], k[0], v[0], g[0], S0[0], 2.0 ** -15), v)
+
+
+@pytest.mark.parametrize("T", [5000, 9000])
+def test_prefill_f16_long(pkg, T):
+    """Cut in time, and sequences of many chunks, at the shape whose K has one stage."""
+    d, io = 128, torch.float16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, T, gmin=-0.02)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), scale=d ** -0.5, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), d ** -0.5)
+    check_f16_rows(o[0].cpu(), ref, v)
+    check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0, -2000:], v[0])
