@@ -118,7 +118,8 @@ struct Layout {
   static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
   static constexpr int kFirst = kGate + 2 * kGateStage;    // per value column, a byte: see Bars::bad
   static constexpr int kShift = kFirst + 128;              // f16: x of V'' per value column, by chunk, a byte
-  static constexpr int kBars = kShift + 2 * 128;
+  static constexpr int kRow = kShift + 2 * 128;            // f16: y of P per row, by chunk, a byte
+  static constexpr int kBars = kRow + 2 * 128;
   static constexpr int kBytes = kBars + 352;
   static_assert(kBytes <= 232448, "shared memory");
 };
@@ -414,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.ds_free, 8);
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
-    mbar_init(&bar.pv_done, 1);
+    mbar_init(&bar.pv_done, BF16 || !FULL ? 1 : 2);
     mbar_init(&bar.ds_done, BF16 ? 1 : 2);
     mbar_init(&bar.s_ready, 8);
     mbar_init(&bar.o_free, 4);
@@ -455,14 +456,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int form = bar.form[st];
       const float own = G[row];  // e^(-G_i) or e^(R - G_i) (bf16: 2^pow of it), or G_i
       const float Gi = form == kNearBlock ? bar.ref[st][warp] + (BF16 ? p.pow : 0.f) - __log2f(own) : own;  // (not kNear)
-      const float f = a.scale * (form == kNear ? __frcp_rn(own) : ex2(Gi));
+      float f = a.scale * (form == kNear ? __frcp_rn(own) : ex2(Gi));
       // SC takes Q as it is.  bf16, and not kFar: so does QS; O then lacks the row's
       // factor, and P leaves it out too: the epilogue applies it.  (kNearBlock: a factor
       // below 2^-kLeast is taken as that; P carries the rest of it, and of the state
       // before the chunk so little arrives that it makes no difference.)  Else P carries
-      // the row's factor, which its type could not do without, and QS takes Q' = scale
-      // e^G Q written over Q: in bf16, whose range it needs, and with f16 I/O in two
-      // parts of it, the lower one over the scores that P leaves free.
+      // the row's factor, and QS takes Q' = scale e^G Q written over Q: in bf16, whose
+      // range it needs, and with f16 I/O in two parts of it, the lower one over the
+      // scores that P leaves free.  f16 does not have P's range either: both are taken
+      // times 2^-y, y by the row's largest of P, and the epilogue applies 2^y.
       const bool by_block = BF16 && form == kNearBlock, plain_q = BF16 && form != kFar;
       const auto queries = [&](bool scaled) {
 #pragma unroll 1
@@ -506,46 +508,66 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!BF16 && (ok = wait(&bar.sc_done, c & 1))) tc::fence_after_sync();
       if (!ok) break;
-      // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
+      // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16);
+      // in f16 a first round finds the row's largest
+      float most = 0.f, shrink = 1.f;
 #pragma unroll 1
-      for (int b = 0; b < 4; ++b) {
-        uint32_t u[16];
-        if (b <= warp) {
-          // the loads first: shared memory answers late while the products read it
-          float x[2][16], d[32];
-          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32, x[0]);
-          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
+      for (int round = BF16; round < 2; ++round) {
+#pragma unroll 1
+        for (int b = 0; b < (round ? 4 : warp + 1); ++b) {
+          uint32_t u[16];
+          if (b <= warp) {
+            // the loads first: shared memory answers late while the products read it
+            float x[2][16], d[32];
+            tc::tmem_ld16(tmem + lanes + kTmSC + b * 32, x[0]);
+            tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
-          if (form == kFar) {
+            for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
+            if (form == kFar) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
-          } else if (by_block) {
-            // the block's factor in two steps of at most 2^kNear, or the row's as well
-            // (its root, twice: the whole may pass the range of a float where d is small)
-            const float r = ex2(0.5f * (Gi - fmaxf(Gi, -kLeast) - bar.ref[st][b]));
+              for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
+            } else if (by_block) {
+              // the block's factor in two steps of at most 2^kSpan, or the row's as well
+              // (its root, twice: the whole may pass the range of a float where d is small)
+              const float r = ex2(0.5f * (Gi - fmaxf(Gi, -kLeast) - bar.ref[st][b]));
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
-          } else if (!BF16) {
-            const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
+              for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
+            } else if (!BF16) {
+              const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] *= r;
+              for (int e = 0; e < 32; ++e) d[e] *= r;
+            }
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) d[e] *= x[e >> 4][e & 15];
+            if (b == warp) {  // on the diagonal
+#pragma unroll
+              for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
+            }
+            if (!BF16) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(d[e]));
+#pragma unroll
+              for (int e = 0; e < 32; ++e) d[e] *= shrink;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = tc::pack2<BF16>(d[2 * e], d[2 * e + 1]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = 0;
           }
-          tc::tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; ++e) d[e] *= x[e >> 4][e & 15];
-          if (b == warp) {  // on the diagonal
-#pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = tc::pack2<BF16>(d[2 * e], d[2 * e + 1]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) u[e] = 0;
+          if (round) tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
         }
-        tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
+        if (!round) {
+          // The row's largest of P 2^-y lies in [2^13, 2^14).  Q' S and Q' 2^-y bound y from
+          // below; for the second of them, only rows of P that are zero come so low.
+          const int y = max(max(static_cast<int>(__float_as_uint(most) >> 23) - 127 - 13, -64),
+                            static_cast<int>(__float_as_uint(fabsf(f)) >> 23) - 127 - 90);
+          shrink = __uint_as_float(static_cast<uint32_t>(127 - y) << 23);
+          smem[L::kRow + st * 128 + row] = static_cast<unsigned char>(y);
+        }
       }
+      f *= shrink;
       if (!BF16) queries(true);
       tc::tmem_wait_st();
       tc::fence_before_sync();
@@ -680,6 +702,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       unsigned char* o = smem + L::kO;
       if (!wait(&bar.pv_done, c & 1, &bar.o_stored, (c & 1) ^ 1, &bar.v_ready[1], c & 1)) return false;
       tc::fence_after_sync();
+      if (!BF16) {
+        const int y = static_cast<signed char>(smem[L::kRow + (c & 1) * 128 + row]);
+        factor = __uint_as_float(static_cast<uint32_t>(127 + y) << 23);
+      }
 #pragma unroll 1
       for (int b = 0; b < BV / 32; ++b) {
         float x[2][16];
@@ -756,12 +782,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         if (!(ok = parts(c, half))) break;
         if (half) {
-          if (FULL) {
+          if (FULL && BF16) {
             const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];
             const int form = bar.form[st];
             factor = 1.f;
-            if (BF16 && form == kNear) factor = a.scale * __frcp_rn(own);
-            if (BF16 && form == kNearBlock) {
+            if (form == kNear) factor = a.scale * __frcp_rn(own);
+            if (form == kNearBlock) {
               const float Gi = bar.ref[st][quarter] + p.pow - __log2f(own);
               factor = p.rest * ex2(fmaxf(Gi, -kLeast));
             }
@@ -1068,6 +1094,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kC / 16; ++s)
           tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
         tc::commit(&bar.pv_done);
+        if (!BF16) mbar_arrive(&bar.pv_done);  // (hands R's shifts on to V)
       }
       tc::commit(&bar.empty[kTileV][st]);
     }

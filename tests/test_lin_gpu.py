@@ -745,3 +745,61 @@ def test_prefill_f16_long(pkg, T):
     ref = steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), d ** -0.5)
     check_f16_rows(o[0].cpu(), ref, v)
     check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0, -2000:], v[0])
+
+
+def f16_size(x, most):
+    return (x / x.abs().max() * most).to(torch.float16)
+
+
+def check_f16_range(o, ref):
+    """check_f16_rows where P passes f16's range: its terms below 2^-39 of the row's largest may be lost, 128 of them;
+    no value of v is much larger than those that the row's largest scores meet, hence 2^-30 of the sum."""
+    ro, _, oa, _ = ref
+    u = half_step(torch.float16)
+    fits = ro.abs() < 65000
+    assert float(fits.double().mean()) > 0.9
+    tol = u * ro.abs() + 2.0 ** -25 + (u + 2.0 ** -16 + 64 * E) * oa + 2.0 ** -30 * oa.amax(2, keepdim=True)
+    assert bool(((o.double() - ro).abs() <= tol)[fits].all()), float(((o.double() - ro).abs() / tol)[fits].max())
+
+
+@pytest.mark.parametrize("scale,vmax", [(1.0, 2.0 ** -20), (2.0 ** 40, 0.0), (2.0 ** -30, 1.0), (2.0 ** -45, 6e4), (-(2.0 ** -60), 6e4)])
+@pytest.mark.parametrize("gmin", [0.0, -0.2, -2.0])
+def test_prefill_f16_scores_beyond_its_range(pkg, gmin, scale, vmax):
+    """Queries and keys near f16's largest: scores of up to 2^71, with outputs that f16 holds; and scores so small
+    that f16 would hold none of them."""
+    T, d, io = 200, 64, torch.float16
+    gen = torch.Generator().manual_seed(65)
+    q, k = (f16_size(torch.randn(1, T, 1, d, generator=gen), 6e4) for _ in range(2))
+    v = f16_size(torch.randn(1, T, 2, d, generator=gen), max(vmax, 2.0 ** -24)) * (vmax > 0)
+    g = torch.rand(1, T, 2, generator=gen) * gmin
+    S0 = torch.randn(1, 2, d, d, generator=gen) * 2.0 ** -20 / scale * (vmax == 0)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=scale, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], S0[0], scale)
+    check_f16_range(o[0].cpu(), ref)
+    u = half_step(io)
+    # (2^-126, fp32's smallest normal number: a state of 2^-60 that decays by 2^-288 is none of fp32's)
+    tol = (u * u + 64 * E) * ref[3] + 2.0 ** -32 * ref[3].amax(1, keepdim=True) + 2.0 ** -126
+    assert bool(((S[0].cpu().double() - ref[1]).abs() <= tol).all())
+
+
+def test_prefill_f16_growing_gates(pkg):
+    """Scores that growing gates take beyond f16's range, with outputs inside it."""
+    T, d, io = 120, 64, torch.float16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 66, gmin=0.25)
+    v = (v.float() * 2.0 ** -18).to(io)
+    v[:, 8:] = 0
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), check=True)
+    check_f16_range(o[0].cpu(), steps(q[0], k[0], v[0], g[0], torch.zeros(2, d, d), 1.0))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 100, 2.0 ** -100, 0.0])
+def test_prefill_f16_rows_without_scores(pkg, scale):
+    """Keys of zero: only the state before is read, at any scale."""
+    T, d, io = 140, 64, torch.float16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 67, gmin=-0.1)
+    k[:] = 0
+    S0 = torch.randn(1, 2, d, d, generator=torch.Generator().manual_seed(68)) / (scale or 1.0)
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=scale, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], S0[0], scale)
+    check_f16_range(o[0].cpu(), ref)
+    assert bool(((S[0].cpu().double() - ref[1]).abs() <= 64 * E * ref[3] + 2.0 ** -126).all())  # (fp32's smallest)
