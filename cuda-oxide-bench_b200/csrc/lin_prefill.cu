@@ -42,9 +42,10 @@
 // state that QS takes, each rounded to bf16 once, give the rest).
 //
 // A value of V that is not finite belongs to the rows from its own on, but P V would
-// bring it to the earlier ones of its chunk, as 0 x NaN.  V notices it while it makes
-// V'' and puts zero in its place in the tile, and the epilogue writes NaN into its
-// column from its row on.
+// bring it to the earlier ones of its chunk, as 0 x NaN.  It makes its column's dS NaN
+// (its lower part is), which S sees; PV waits for that, the MMA warp puts zero in its
+// place in the tile, and the epilogue writes NaN into its column from its row on.  (4% of
+// the time, at d = 64 9%; a test of each value by V took 6% and 14%.)
 //
 // What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 to 120 us, 403 MB,
 // so 3.4 TB/s or 0.52 of the measured copy; 97 us in a burst, before the power limit
@@ -135,9 +136,10 @@ struct Bars {
   float gamma[2];
   float ref[2][4];  // R_b
   int form[2];      // kNear, kNearBlock, kFar
-  // by chunk and V warp: some value of its columns is not finite, and kFirst holds the
-  // first token of which that is so for each of them (kC: none)
-  alignas(8) uint8_t bad[2][4];
+  // 1 + the last chunk in which dS is NaN; kFirst then holds, per value column, the first
+  // token whose value is not finite (kC: none)
+  int bad;
+  int call;         // the MMA thread to the rest of its warp
   uint32_t tmem;
 };
 static_assert(sizeof(Bars) <= 352, "barriers");
@@ -383,6 +385,37 @@ __device__ __forceinline__ bool wait(uint64_t* b0, uint32_t p0, uint64_t* b1, ui
   return __all_sync(0xffffffffu, wait1(b0, p0, b1, p1, b1, p1));
 }
 
+// A warp: puts zero in the place of what is not finite in a tile of V and leaves the first
+// token of which that is so in first[column] (kC: none; dS is NaN for a key's sake too).
+__device__ __noinline__ void clear_values(unsigned char* tile, int columns, uint32_t exponent, unsigned char* first) {
+  for (int x = (threadIdx.x & 31) * 2; x < columns; x += 64) {
+    unsigned char* at = tile + (x >> 6) * kTile + (x & 7) * 2;
+    int first0 = kC, first1 = kC;
+#pragma unroll 4
+    for (int t = kC - 1; t >= 0; --t) {
+      uint32_t* v = reinterpret_cast<uint32_t*>(at + tc::sw128_offset(t, (x & 63) >> 3));
+      const uint32_t u = *v;
+      const bool bad0 = (u & exponent) == exponent, bad1 = (u >> 16 & exponent) == exponent;
+      if (bad0) first0 = t;
+      if (bad1) first1 = t;
+      if (bad0 || bad1) *v = (bad0 ? 0u : u & 0xffffu) | (bad1 ? 0u : u & 0xffff0000u);
+    }
+    first[x] = static_cast<unsigned char>(first0);
+    first[x + 1] = static_cast<unsigned char>(first1);
+  }
+  tc::fence_proxy_async();
+  __syncwarp();
+}
+
+// A thread with the row `row` of a tile of O: NaN in the columns that a value of that row
+// or one before belongs to which is not finite.
+__device__ __noinline__ void mark_row(unsigned char* tile, int row, int columns, const unsigned char* first) {
+#pragma unroll 1
+  for (int x = 0; x < columns; ++x)
+    if (row >= first[x])
+      *reinterpret_cast<uint16_t*>(tile + (x >> 6) * kTile + tc::sw128_offset(row, (x & 63) >> 3) + (x & 7) * 2) = 0x7fff;
+}
+
 // FULL: everything.  Else only what a piece adds to the state and its decay, from k,
 // v and the gates; the tensor memory that is free then is a second place for V''.
 template <int DK, int BV, typename IO, bool FULL>
@@ -415,7 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.ds_free, 8);
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
-    mbar_init(&bar.pv_done, BF16 || !FULL ? 1 : 2);
+    mbar_init(&bar.pv_done, FULL ? 2 : 1);
     mbar_init(&bar.ds_done, BF16 ? 1 : 2);
     mbar_init(&bar.s_ready, 8);
     mbar_init(&bar.o_free, 4);
@@ -423,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.o_stored, 1);
     mbar_init(&bar.zeroed, 4);
     mbar_init(&bar.drain, 1);
-    *reinterpret_cast<uint64_t*>(bar.bad) = 0;  // (warps without columns write none)
+    bar.bad = 0;
     fence_mbar_init();
   }
   if (tid < 4) prefetch_map(tid == 0 ? &map_q : tid == 1 ? &map_k : tid == 2 ? &map_v : &map_o);
@@ -583,7 +616,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int quarter = warp - kWarpV, row = quarter * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const bool has_rows = quarter * 32 < BV;
-    int first = kC;  // the first token of the chunk whose value in column `row` is not finite
     // Of this lane's tokens 2 l, 2 l + 1 and 2 l + 8, 2 l + 9 of each 16 of a half, l = lane % 4:
     // (hi, lo) of w for both tokens of a pair, or (f16) w of each
     const auto weights = [&](int st, int half, uint32_t (&ww)[4][4]) {
@@ -638,7 +670,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     // tokens [64 half, 64 half + 64) of chunk c: both parts
     const auto parts = [&](int c, int half) {
       const int st = c & 1;
-      if (!half) first = kC;
       if (has_rows) {
         if (!BF16 && !half) find_shifts(st);
         uint32_t ww[4][4], r[2][4][4];
@@ -646,7 +677,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // all loads first (unrolled 98.2 against 99.5 us; at d = 64 37.9 against 40.7)
         values(st, half, 0, r[0]);
         values(st, half, 1, r[1]);
-        uint32_t bad = 0;  // 0 v: zero, or NaN where v is not finite
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t hi[16], lo[16];
@@ -662,45 +692,24 @@ __global__ void __launch_bounds__(kThreads, 1)
               hi[e] = tc::pack2<BF16>(x, y);
               lo[e] = tc::pack2<BF16>(x - tc::unpack_lo<BF16>(hi[e]), y - tc::unpack_hi<BF16>(hi[e]));
             }
-            if (FULL) bad = tc::fma2<BF16>(v, 0, bad);
           }
           const uint32_t to = tmem + lanes + (static_cast<uint32_t>(i * 16) << 16) + (FULL || half ? kTmV : kTmSC);
           tc::tmem_st_16x128b_x8(to, lo);
           tc::tmem_st_16x128b_x8(to + 32, hi);
         }
         tc::tmem_wait_st();
-        if (FULL && __any_sync(0xffffffffu, bad != 0)) {
-          constexpr uint32_t kExponent = BF16 ? 0x7f80 : 0x7c00;
-          unsigned char* column = smem + L::kV + st * L::kVTile + (row >> 6) * kTile + (row & 7) * 2;
-#pragma unroll 1
-          for (int t = half * 64; t < half * 64 + 64; ++t) {
-            uint16_t* x = reinterpret_cast<uint16_t*>(column + tc::sw128_offset(t, (row & 63) >> 3));
-            if ((*x & kExponent) == kExponent) {
-              first = min(first, t);
-              *x = 0;
-            }
-          }
-          tc::fence_proxy_async();
-        }
-        if (FULL && half) {
-          const bool any = __any_sync(0xffffffffu, first < kC);
-          if (any) {  // once every warp has read the marks of the chunk before
-            if (!wait(&bar.o_free, (c & 1) ^ 1)) return false;
-            smem[L::kFirst + row] = static_cast<unsigned char>(first);
-          }
-          if (lane == 0) bar.bad[st][quarter] = any;
-        }
       }
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.v_ready[half]);
-      return true;
     };
     // O of chunk c: a token per thread, times the row's factor, packed into shared memory
     float factor = 1.f;
     const auto output = [&](int c) {
       unsigned char* o = smem + L::kO;
-      if (!wait(&bar.pv_done, c & 1, &bar.o_stored, (c & 1) ^ 1, &bar.v_ready[1], c & 1)) return false;
+      if (!wait(&bar.pv_done, c & 1, &bar.o_stored, (c & 1) ^ 1)) return false;
+      uint32_t bad;  // asked for early
+      asm volatile("ld.shared.b32 %0, [%1];" : "=r"(bad) : "r"(smem_u32(&bar.bad)));
       tc::fence_after_sync();
       if (!BF16) {
         const int y = static_cast<signed char>(smem[L::kRow + (c & 1) * 128 + row]);
@@ -721,12 +730,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                      tc::pack2<BF16>(factor * y[6], factor * y[7]));
         }
       }
-      if (*reinterpret_cast<const uint32_t*>(bar.bad[c & 1])) {
-#pragma unroll 1
-        for (int i = 0; i < BV; ++i)
-          if (bar.bad[c & 1][i >> 5] && row >= smem[L::kFirst + i])
-            *reinterpret_cast<uint16_t*>(o + (i >> 6) * kTile + tc::sw128_offset(row, (i & 63) >> 3) + (i & 7) * 2) = 0x7fff;
-      }
+      if (bad == c + 1) mark_row(o, row, BV, smem + L::kFirst);
       tc::fence_before_sync();
       tc::fence_proxy_async();
       __syncwarp();
@@ -780,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int before = FULL ? step - 1 : step - 2;
         if (before >= 0 && !(ok = wait(&bar.v_free[before & 1], (before >> 1) & 1))) break;
         tc::fence_after_sync();
-        if (!(ok = parts(c, half))) break;
+        parts(c, half);
         if (half) {
           if (FULL && BF16) {
             const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];
@@ -822,14 +826,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (has_rows) {
           const int x = BF16 ? 0 : static_cast<signed char>(smem[L::kShift + st * 128 + row]);
           const float grow = __uint_as_float(static_cast<uint32_t>(127 + x) << 23);
+          bool bad = false;
 #pragma unroll
           for (int b = 0; b < kN / 16; ++b) {
             float d[16];
             tc::tmem_ld16(tmem + lanes + kTmDS + half * kN + b * 16, d);
             tc::tmem_wait_ld();
+            if (b == 0) bad = isnan(d[0]);
 #pragma unroll
             for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], BF16 ? d[e] : grow * d[e]);
           }
+          if (FULL && __any_sync(0xffffffffu, bad) && lane == 0) bar.bad = c + 1;
         }
         tc::fence_before_sync();
         __syncwarp();
@@ -1020,8 +1027,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       bulk_wait_all();
     }
-  } else if (warp == kWarpMma && tc::elect_one()) {
-    // ------------------------------------------------ MMA
+  } else if (warp == kWarpMma && !tc::elect_one()) {
+    // the other lanes, for which bar.call holds a chunk that wants clear_values, at last 0
+    for (;;) {
+      __syncwarp();
+      const int c = *static_cast<volatile int*>(&bar.call) - 1;
+      if (!FULL || c < 0) break;
+      clear_values(smem + L::kV + (c & 1) * L::kVTile, BV, BF16 ? 0x7f80 : 0x7c00, smem + L::kFirst);
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------ MMA: the elected lane
     constexpr uint32_t kIdSC = tc::idesc_f16(128, kC, false, false, BF16);
     constexpr uint32_t kIdDS = tc::idesc_f16(128, DK, false, true, BF16);
     constexpr uint32_t kIdQS = tc::idesc_f16(128, BV, false, false, true);
@@ -1077,9 +1092,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&bar.empty[kTileK][kst]);
 
       if constexpr (FULL) {
-        if (BF16) ok = wait1(&bar.p_ready, c & 1);
-        else ok = wait1(&bar.p_ready, c & 1, &bar.s_ready, c & 1, &bar.o_free, (c & 1) ^ 1);
+        ok = wait1(&bar.p_ready, c & 1, &bar.ds_free, c & 1, BF16 ? &bar.p_ready : &bar.s_ready, c & 1);
+        if (!BF16 && ok) ok = wait1(&bar.o_free, (c & 1) ^ 1);
         if (!ok) break;
+        if (*static_cast<volatile int*>(&bar.bad) == c + 1) {
+          bar.call = c + 1;
+          __syncwarp();
+          clear_values(smem + L::kV + st * L::kVTile, BV, BF16 ? 0x7f80 : 0x7c00, smem + L::kFirst);
+        }
         tc::fence_after_sync();
         if constexpr (!BF16) {  // lower part of Q', lower part of S^T, the upper ones
 #pragma unroll
@@ -1094,7 +1114,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kC / 16; ++s)
           tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
         tc::commit(&bar.pv_done);
-        if (!BF16) mbar_arrive(&bar.pv_done);  // (hands R's shifts on to V)
+        mbar_arrive(&bar.pv_done);  // (hands kFirst, and in f16 R's shifts, on to V)
       }
       tc::commit(&bar.empty[kTileV][st]);
     }
@@ -1102,6 +1122,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&bar.drain);
       wait1(&bar.drain, 0);
     }
+    bar.call = 0;
+    __syncwarp();
   }
   // a wait ran out: for a free slot, or for what the other warps do
   if (!ok) report(status, warp == kWarpTma || warp == kWarpGate ? GDN_DEVERR_EMPTY_TIMEOUT : GDN_DEVERR_MMA_TIMEOUT);
