@@ -26,7 +26,7 @@
 //   PV  O    += P V                then V applies the rows' factors and stages O
 // D0 and D1 lie between the others so that the tensor cores have work while R and
 // V prepare the next operand.  With f16 I/O QS, which R makes ready last, comes after
-// D1, and is three products: queries and state each in two parts of bf16, which has
+// PV, and is three products: queries and state each in two parts of bf16, which has
 // the range for them, 2^-17 off.  All five take A from TMEM: a product with both
 // operands in shared memory reads it at its full rate, and other warps' reads then
 // take five times as long (4 ldmatrix.x4: 726 cycles against 141).
@@ -578,8 +578,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
             }
             if (!BF16) {
+              if (!round) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(d[e]));
+                for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(d[e]));
+                continue;
+              }
 #pragma unroll
               for (int e = 0; e < 32; ++e) d[e] *= shrink;
             }
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 16; ++e) u[e] = 0;
           }
-          if (round) tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
+          tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
         }
         if (!round) {
           // The row's largest of P 2^-y lies in [2^13, 2^14).  Q' S and Q' 2^-y bound y from
@@ -600,15 +603,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           smem[L::kRow + st * 128 + row] = static_cast<unsigned char>(y);
         }
       }
-      f *= shrink;
-      if (!BF16) queries(true);
       tc::tmem_wait_st();
       tc::fence_before_sync();
       __syncwarp();
       if (lane == 0) {
-        if (!BF16) mbar_arrive(&bar.empty[kTileQ][0]);
         mbar_arrive(&bar.p_ready);
         mbar_arrive(&bar.gempty[st]);
+      }
+      if (!BF16) {
+        f *= shrink;
+        queries(true);
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&bar.q2_ready);
+          mbar_arrive(&bar.empty[kTileQ][0]);
+        }
       }
     }
   } else if (warp >= kWarpV && warp < kWarpS) {
@@ -1092,8 +1103,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&bar.empty[kTileK][kst]);
 
       if constexpr (FULL) {
-        ok = wait1(&bar.p_ready, c & 1, &bar.ds_free, c & 1, BF16 ? &bar.p_ready : &bar.s_ready, c & 1);
-        if (!BF16 && ok) ok = wait1(&bar.o_free, (c & 1) ^ 1);
+        ok = wait1(&bar.p_ready, c & 1, &bar.ds_free, c & 1, BF16 ? &bar.p_ready : &bar.o_free, BF16 ? c & 1 : (c & 1) ^ 1);
         if (!ok) break;
         if (*static_cast<volatile int*>(&bar.bad) == c + 1) {
           bar.call = c + 1;
@@ -1101,22 +1111,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           clear_values(smem + L::kV + st * L::kVTile, BV, BF16 ? 0x7f80 : 0x7c00, smem + L::kFirst);
         }
         tc::fence_after_sync();
+#pragma unroll
+        for (int s = 0; s < kC / 16; ++s)
+          tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, BF16 || s > 0);
+        tc::commit(&bar.empty[kTileV][st]);
         if constexpr (!BF16) {  // lower part of Q', lower part of S^T, the upper ones
+          if (!(ok = wait1(&bar.q2_ready, c & 1, &bar.s_ready, c & 1, &bar.s_ready, c & 1))) break;
+          tc::fence_after_sync();
 #pragma unroll
           for (int part = 0; part < 3; ++part)
 #pragma unroll
             for (int s = 0; s < DK / 16; ++s)
               tc::mma_tmem_a(kTmO, (part ? kTmQ : kTmQLow) + s * 8, sT + along(s, L::kSBlock) + (part == 1 ? L::kSPart >> 4 : 0),
-                             kIdQS, part || s > 0);
+                             kIdQS, true);
           tc::commit(&bar.qs_done);
         }
-#pragma unroll
-        for (int s = 0; s < kC / 16; ++s)
-          tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, true);
         tc::commit(&bar.pv_done);
         mbar_arrive(&bar.pv_done);  // (hands kFirst, and in f16 R's shifts, on to V)
+      } else {
+        tc::commit(&bar.empty[kTileV][st]);
       }
-      tc::commit(&bar.empty[kTileV][st]);
     }
     if (!ok) {  // products in flight end before the tensor memory is released
       tc::commit(&bar.drain);
