@@ -73,7 +73,6 @@ constexpr int kTile = kC * 128;     // bytes of a [128][64] 16-bit tile
 constexpr int kThreads = 20 * 32;
 constexpr int kWarpV = 4, kWarpS = 8, kWarpTma = 16, kWarpGate = 17, kWarpMma = 18, kWarpStore = 19;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr uint32_t kWaitTries = 1u << 18;
 // Up to so many sequences of a packed batch are put in order of length: 24 ragged ones
 // take 89.6 us and not 98, 32 of 20000 tokens 192 and not 203; 200, whose order takes
 // each of 3200 CTAs 2 us to find, 409 and not 365.
@@ -335,14 +334,22 @@ __device__ __forceinline__ float log2_gate(float g) {
   return x < kLowest ? kLowest : x;
 }
 
-// Waits for a phase; false after about a second.  A try sleeps in the barrier unit
-// until the phase completes or 8000 cycles have gone by (measured; the hint makes no
-// difference), so the tries are what is counted: two dozen copies of this share the
-// instruction cache with the roles' loops, and no clock is read.  wait1() is for one
-// thread; wait() for a whole warp, whose lanes all get the same answer.
+// The lower half of the clock, in ns: two dozen copies of the waits below share the
+// instruction cache with the roles' loops.  (Read after the first failed try only: 104.7
+// us in bursts of the batch case; the whole of it 103.5; this 101.9.)
+__device__ __forceinline__ uint32_t now_ns() {
+  uint32_t t;
+  asm volatile("mov.u32 %0, %%globaltimer_lo;" : "=r"(t));
+  return t;
+}
+static_assert(kWaitLimitNs < 1ull << 31, "half a clock");
+
+// Waits for a phase; false after kWaitLimitNs.  wait1() is for one thread; wait() for a
+// whole warp, whose lanes all get the same answer.
 __device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity) {
   const uint32_t at = smem_u32(bar);
-  uint32_t ok, tries = kWaitTries;
+  const uint32_t t0 = now_ns();
+  uint32_t ok;
   do {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
@@ -351,7 +358,7 @@ __device__ __forceinline__ bool wait1(uint64_t* bar, uint32_t parity) {
         : "=r"(ok)
         : "r"(at), "r"(parity)
         : "memory");
-  } while (!ok && --tries);
+  } while (!ok && now_ns() - t0 < static_cast<uint32_t>(kWaitLimitNs));
   return ok != 0;
 }
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
@@ -362,7 +369,8 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
 // barrier parity 1 counts as complete: that of the chunk before the first.
 __device__ __forceinline__ bool wait1(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2) {
   const uint32_t at0 = smem_u32(b0), at1 = smem_u32(b1), at2 = smem_u32(b2);
-  uint32_t ok, tries = kWaitTries;
+  const uint32_t t0 = now_ns();
+  uint32_t ok;
   do {
     asm volatile(
         "{\n\t.reg .pred p, q, r;\n\t"
@@ -375,7 +383,7 @@ __device__ __forceinline__ bool wait1(uint64_t* b0, uint32_t p0, uint64_t* b1, u
         : "=r"(ok)
         : "r"(at0), "r"(p0), "r"(at1), "r"(p1), "r"(at2), "r"(p2)
         : "memory");
-  } while (!ok && --tries);
+  } while (!ok && now_ns() - t0 < static_cast<uint32_t>(kWaitLimitNs));
   return ok != 0;
 }
 __device__ __forceinline__ bool wait(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, uint64_t* b2, uint32_t p2) {
