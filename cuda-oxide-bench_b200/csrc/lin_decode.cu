@@ -173,23 +173,26 @@ int validate(const lin_decode_args_t* a) {
   if (a->dk != 64 && a->dk != 128 && a->dk != 256) return GDN_ERR_SHAPE;
   if (a->dv < 64 || a->dv % 64) return GDN_ERR_SHAPE;
   const int64_t page = static_cast<int64_t>(a->Hv) * a->dk * a->dv;
-  if (page > INT32_MAX || a->state_in_sp < page || a->state_out_sp < page) return GDN_ERR_SHAPE;
+  // the stride of an axis of one is free
+  const bool rows = a->B > 1, many = a->pages > 1;
+  if (page > INT32_MAX || (many && (a->state_in_sp < page || a->state_out_sp < page))) return GDN_ERR_SHAPE;
   if (a->io_dtype != GDN_DT_BF16 && a->io_dtype != GDN_DT_F16) return GDN_ERR_DTYPE;
   if (!dtype_valid(a->g_dtype)) return GDN_ERR_DTYPE;
   if (a->gate_kind != GDN_GATE_LOG && a->gate_kind != GDN_GATE_LINEAR) return GDN_ERR_DTYPE;
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->state_in) ||
       !aligned16(a->state_out))
     return GDN_ERR_ALIGN;
-  if (!stride_ok(a->q_sb, 2) || !stride_ok(a->q_sh, 2) || !stride_ok(a->k_sb, 2) || !stride_ok(a->k_sh, 2) ||
-      !stride_ok(a->v_sb, 2) || !stride_ok(a->v_sh, 2) || !stride_ok(a->o_sb, 2) || !stride_ok(a->o_sh, 2) ||
-      !stride_ok(a->state_in_sp, 4) || !stride_ok(a->state_out_sp, 4))
+  if (rows && (!stride_ok(a->q_sb, 2) || !stride_ok(a->k_sb, 2) || !stride_ok(a->v_sb, 2) || !stride_ok(a->o_sb, 2)))
     return GDN_ERR_ALIGN;
-  if ((a->B > 1 && a->o_sb == 0) || (a->Hv > 1 && a->o_sh == 0)) return GDN_ERR_SHAPE;  // rows of o on one another
+  if (a->Hqk > 1 && (!stride_ok(a->q_sh, 2) || !stride_ok(a->k_sh, 2))) return GDN_ERR_ALIGN;
+  if (a->Hv > 1 && (!stride_ok(a->v_sh, 2) || !stride_ok(a->o_sh, 2))) return GDN_ERR_ALIGN;
+  if (many && (!stride_ok(a->state_in_sp, 4) || !stride_ok(a->state_out_sp, 4))) return GDN_ERR_ALIGN;
+  if ((rows && a->o_sb == 0) || (a->Hv > 1 && a->o_sh == 0)) return GDN_ERR_SHAPE;  // rows of o on one another
   if (a->state_in != a->state_out) {
     const float *i1 = a->state_in + (a->pages - 1) * a->state_in_sp + page;
     const float *o1 = a->state_out + (a->pages - 1) * a->state_out_sp + page;
     if (a->state_in < o1 && a->state_out < i1) return GDN_ERR_SHAPE;
-  } else if (a->state_in_sp != a->state_out_sp) {
+  } else if (many && a->state_in_sp != a->state_out_sp) {
     return GDN_ERR_SHAPE;
   }
   return GDN_OK;

@@ -1333,7 +1333,8 @@ int validate(const lin_prefill_args_t* a) {
   if (a->dv < 64 || a->dv % 64) return GDN_ERR_SHAPE;
   if (a->T > INT32_MAX - 2 * kC) return GDN_ERR_SHAPE;
   const int64_t page = static_cast<int64_t>(a->Hv) * a->dk * a->dv;
-  if (page > INT32_MAX || a->final_sp < page || (a->initial_state && a->initial_sp < page)) return GDN_ERR_SHAPE;
+  const bool many = a->pages > 1;  // the stride of an axis of one is free
+  if (page > INT32_MAX || (many && (a->final_sp < page || (a->initial_state && a->initial_sp < page)))) return GDN_ERR_SHAPE;
   if (a->io_dtype != GDN_DT_BF16 && a->io_dtype != GDN_DT_F16) return GDN_ERR_DTYPE;
   if (!dtype_valid(a->g_dtype)) return GDN_ERR_DTYPE;
   if (!aligned16(a->q) || !aligned16(a->k) || !aligned16(a->v) || !aligned16(a->o) || !aligned16(a->final_state) ||
@@ -1345,16 +1346,17 @@ int validate(const lin_prefill_args_t* a) {
     const int heads = i < 2 ? a->Hqk : a->Hv, B = a->cu_seqlens ? 1 : a->B;
     const int size[3] = {B, a->T, heads};
     for (int j = 0; j < 3; ++j) {
-      if (size[j] > 1 && (st[i][j] < 1 || st[i][j] >= (1ll << 38))) return GDN_ERR_SHAPE;
+      if (size[j] == 1) continue;
+      if (st[i][j] < 1 || st[i][j] >= (1ll << 38)) return GDN_ERR_SHAPE;
       if (!stride_ok(st[i][j], 2)) return GDN_ERR_ALIGN;
     }
   }
-  if (!stride_ok(a->final_sp, 4) || (a->initial_state && !stride_ok(a->initial_sp, 4))) return GDN_ERR_ALIGN;
+  if (many && (!stride_ok(a->final_sp, 4) || (a->initial_state && !stride_ok(a->initial_sp, 4)))) return GDN_ERR_ALIGN;
   if (a->initial_state && a->initial_state != a->final_state) {
     const float* i1 = a->initial_state + (a->pages - 1) * a->initial_sp + page;
     const float* f1 = a->final_state + (a->pages - 1) * a->final_sp + page;
     if (a->initial_state < f1 && a->final_state < i1) return GDN_ERR_SHAPE;
-  } else if (a->initial_state && a->initial_sp != a->final_sp) {
+  } else if (many && a->initial_state && a->initial_sp != a->final_sp) {
     return GDN_ERR_SHAPE;
   }
   return GDN_OK;

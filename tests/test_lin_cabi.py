@@ -267,3 +267,34 @@ def test_cpu_tensors_are_refused(pkg):
                  lambda: pkg.pages_compact(pool, flags)):
         with pytest.raises(pkg.GDNError):
             call()
+
+
+# ------------------------------------------------------- strides of axes of one entry
+
+
+ONE_D = {"B": 1, "Hqk": 1, "Hv": 1, "pages": 1, "state_in_sp": 1, "state_out_sp": 3,
+         **{x: 1 for x in ("q_sb", "q_sh", "k_sb", "k_sh", "v_sb", "v_sh", "o_sb", "o_sh")}}
+ONE_P = {"B": 1, "T": 1, "Hqk": 1, "Hv": 1, "pages": 1, "final_sp": 1, "initial_sp": 3,
+         **{x + y: 1 for x in ("q_s", "k_s", "v_s", "o_s") for y in "bth"}}
+
+
+@pytest.mark.skipif(has_gpu(), reason="checks the no-device path")
+def test_strides_of_axes_of_one_entry_are_free(pkg):
+    L = pkg._lib.load()
+    assert L.lin_decode_launch(ctypes.byref(decode_args(pkg, **ONE_D)), None) == 6
+    assert L.lin_prefill_launch(ctypes.byref(prefill_args(pkg, **ONE_P)), None) == 6
+    # packed: one batch, whatever the number of sequences
+    a = prefill_args(pkg, cu_seqlens=BASE, q_sb=1, k_sb=-3, v_sb=5, o_sb=0)
+    assert L.lin_prefill_launch(ctypes.byref(a), None) == 6
+
+
+@pytest.mark.parametrize("one,over", [(ONE_D, {"B": 2, "pages": 2, "state_in_sp": 1 << 16, "state_out_sp": 1 << 16}), (ONE_D, {"Hv": 2})])
+def test_decode_strides_of_longer_axes_are_checked(pkg, one, over):
+    a = decode_args(pkg, **{**one, **over})
+    assert pkg._lib.load().lin_decode_launch(ctypes.byref(a), None) == 3
+
+
+@pytest.mark.parametrize("over", [{"B": 2, "pages": 2, "final_sp": 1 << 16}, {"T": 2}, {"Hv": 2}])
+def test_prefill_strides_of_longer_axes_are_checked(pkg, over):
+    a = prefill_args(pkg, **{**ONE_P, **over})
+    assert pkg._lib.load().lin_prefill_launch(ctypes.byref(a), None) == 3
