@@ -26,6 +26,16 @@ inline bool stride_ok(int64_t elems, int esize) { return ((elems * esize) & 15) 
 inline int host_dtype_size(int dt) { return dt == GDN_DT_F32 ? 4 : 2; }
 inline bool dtype_valid(int dt) { return dt == GDN_DT_F32 || dt == GDN_DT_BF16 || dt == GDN_DT_F16; }
 
+// Whether two pools of `pages` pages of `page` fp32 elements, `sp` and `sq` elements
+// apart, share no memory: pages of one stride may lie between one another, as the
+// layers of one tensor do.
+inline bool pools_disjoint(const float* p, int64_t sp, const float* q, int64_t sq, int64_t page, int64_t pages) {
+  if (p + (pages - 1) * sp + page <= q || q + (pages - 1) * sq + page <= p) return true;
+  if (sp != sq || pages == 1) return false;
+  const int64_t apart = (p < q ? q - p : p - q) % sp;
+  return apart >= page && sp - apart >= page;
+}
+
 // Encodes (or returns a cached) 2-D fp32 tensor map over a row-major matrix
 // of `rows` x `cols` with a box of `box_rows` x `box_cols`.  Returns GDN_OK or
 // an error code.  The cache is keyed by every argument and guarded by a mutex.

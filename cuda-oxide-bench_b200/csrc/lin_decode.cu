@@ -189,9 +189,7 @@ int validate(const lin_decode_args_t* a) {
   if (many && (!stride_ok(a->state_in_sp, 4) || !stride_ok(a->state_out_sp, 4))) return GDN_ERR_ALIGN;
   if ((rows && a->o_sb == 0) || (a->Hv > 1 && a->o_sh == 0)) return GDN_ERR_SHAPE;  // rows of o on one another
   if (a->state_in != a->state_out) {
-    const float *i1 = a->state_in + (a->pages - 1) * a->state_in_sp + page;
-    const float *o1 = a->state_out + (a->pages - 1) * a->state_out_sp + page;
-    if (a->state_in < o1 && a->state_out < i1) return GDN_ERR_SHAPE;
+    if (!pools_disjoint(a->state_in, a->state_in_sp, a->state_out, a->state_out_sp, page, a->pages)) return GDN_ERR_SHAPE;
   } else if (many && a->state_in_sp != a->state_out_sp) {
     return GDN_ERR_SHAPE;
   }

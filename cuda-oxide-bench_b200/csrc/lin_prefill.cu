@@ -1353,9 +1353,7 @@ int validate(const lin_prefill_args_t* a) {
   }
   if (many && (!stride_ok(a->final_sp, 4) || (a->initial_state && !stride_ok(a->initial_sp, 4)))) return GDN_ERR_ALIGN;
   if (a->initial_state && a->initial_state != a->final_state) {
-    const float* i1 = a->initial_state + (a->pages - 1) * a->initial_sp + page;
-    const float* f1 = a->final_state + (a->pages - 1) * a->final_sp + page;
-    if (a->initial_state < f1 && a->final_state < i1) return GDN_ERR_SHAPE;
+    if (!pools_disjoint(a->initial_state, a->initial_sp, a->final_state, a->final_sp, page, a->pages)) return GDN_ERR_SHAPE;
   } else if (many && a->initial_state && a->initial_sp != a->final_sp) {
     return GDN_ERR_SHAPE;
   }

@@ -298,3 +298,35 @@ def test_decode_strides_of_longer_axes_are_checked(pkg, one, over):
 def test_prefill_strides_of_longer_axes_are_checked(pkg, over):
     a = prefill_args(pkg, **{**ONE_P, **over})
     assert pkg._lib.load().lin_prefill_launch(ctypes.byref(a), None) == 3
+
+
+# ------------------------------------------------------- pools between one another
+
+PAGE = 4 * 128 * 128  # elements of a page of decode_args and prefill_args
+IN = BASE + 4 * (1 << 32)
+
+
+@pytest.mark.parametrize("sp,shift,ok", [
+    (2 * PAGE, PAGE, True), (3 * PAGE, 2 * PAGE, True), (3 * PAGE, PAGE, True), (2 * PAGE, -PAGE, True),
+    (3 * PAGE, 7 * PAGE, True),                             # another layer, some pages on
+    (PAGE, 4 * PAGE, True), (PAGE, -4 * PAGE, True),        # end to end
+    (PAGE, PAGE, False), (3 * PAGE, 3 * PAGE, False),       # the next page of the same layer
+    (2 * PAGE, PAGE - 4, False), (2 * PAGE, PAGE + 4, False), (2 * PAGE + 8, PAGE + 4, True),
+    (2 * PAGE, 4, False),
+])
+def test_pools_that_share_memory(pkg, sp, shift, ok):
+    L = pkg._lib.load()
+    if ok and has_gpu():
+        pytest.skip("checks the no-device path")
+    a = decode_args(pkg, state_in_sp=sp, state_out_sp=sp, state_out=IN + 4 * shift)
+    assert L.lin_decode_launch(ctypes.byref(a), None) == (6 if ok else 2)
+    a = prefill_args(pkg, B=4, T=7, pages=4, initial_sp=sp, final_sp=sp, initial_state=IN + 4 * shift, final_state=IN)
+    assert L.lin_prefill_launch(ctypes.byref(a), None) == (6 if ok else 2)
+
+
+def test_pools_of_unlike_strides_must_lie_apart(pkg):
+    L = pkg._lib.load()
+    a = decode_args(pkg, state_in_sp=2 * PAGE, state_out_sp=4 * PAGE, state_out=IN + 4 * PAGE)
+    assert L.lin_decode_launch(ctypes.byref(a), None) == 2
+    a = prefill_args(pkg, initial_sp=4 * PAGE, final_sp=2 * PAGE, initial_state=IN + 4 * PAGE, final_state=IN)
+    assert L.lin_prefill_launch(ctypes.byref(a), None) == 2

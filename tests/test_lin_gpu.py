@@ -822,3 +822,19 @@ def test_axes_of_one_entry_have_any_stride(pkg):
     want = pkg.lin_decode(q, k, v, g[:, 0], S, check=True)
     q, k, v = (x.as_strided((1, 1, d), (1, 1, 1)) for x in (q, k, v))
     assert torch.equal(pkg.lin_decode(q, k, v, g[:, 0], fin, check=True), want) and torch.equal(fin, S)
+
+
+def test_states_of_one_layer_into_another(pkg):
+    """Layers of one tensor, whose pages lie between one another: out of place, with nothing else written."""
+    B, T, H, d, io = 3, 70, 2, 64, torch.bfloat16
+    layers = torch.randn(B, 3, H, d, d, generator=torch.Generator().manual_seed(70)).to(DEV)
+    before = layers.clone()
+    q, k, v, g = (x.to(DEV) for x in make((B, T), H, H, d, d, io, 71))
+    o, S = pkg.lin_prefill(q, k, v, g, layers[:, 0].clone(), check=True)
+    got, _ = pkg.lin_prefill(q, k, v, g, layers[:, 0], final_state=layers[:, 2], check=True)
+    assert torch.equal(got, o) and torch.equal(layers[:, 2], S) and torch.equal(layers[:, :2], before[:, :2])
+    token = [x[:, 0].contiguous() for x in (q, k, v, g)]
+    want = S.clone()
+    o = pkg.lin_decode(*token, want)
+    assert torch.equal(pkg.lin_decode(*token, layers[:, 2], state_out=layers[:, 1], check=True), o)
+    assert torch.equal(layers[:, 1], want) and torch.equal(layers[:, 2], S) and torch.equal(layers[:, 0], before[:, 0])
