@@ -207,7 +207,7 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
                                       dtype=torch.float32, device=q.device)
     args = (q, k, v, g, initial_state, final_state, out, cu_seqlens, index, scale, _status(dev))
     a = _prefill_args(*args)
-    need = _prefill_workspace(a) if v.shape[1] > _UNCUT else 0
+    need = _prefill_workspace(a, dev) if v.shape[1] > _UNCUT else 0
     if need:
         # from the allocator on the current stream, so that calls on other streams
         # and captured graphs have workspaces of their own
@@ -222,7 +222,11 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
     return out, final_state
 
 
-def _prefill_workspace(args: bytes) -> int:
+def _prefill_workspace(args: bytes, dev: int | None = None) -> int:
+    """What the call needs on device `dev` (the current one), whose SMs decide how it is cut."""
+    if dev is not None and torch.cuda.current_device() != dev:
+        with torch.cuda.device(dev):
+            return _prefill_workspace(args)
     return _lib.load().lin_prefill_workspace_size(
         ctypes.cast(ctypes.c_char_p(args), ctypes.POINTER(_lib.LinPrefillArgs)))
 

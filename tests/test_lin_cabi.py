@@ -330,3 +330,30 @@ def test_pools_of_unlike_strides_must_lie_apart(pkg):
     assert L.lin_decode_launch(ctypes.byref(a), None) == 2
     a = prefill_args(pkg, initial_sp=4 * PAGE, final_sp=2 * PAGE, initial_state=IN + 4 * PAGE, final_state=IN)
     assert L.lin_prefill_launch(ctypes.byref(a), None) == 2
+
+
+def test_workspace_is_asked_for_on_the_tensors_device(pkg, monkeypatch):
+    lin, at, asked = _lin(), [0], []
+
+    class On:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            self.before, at[0] = at[0], self.dev
+
+        def __exit__(self, *_):
+            at[0] = self.before
+
+    class Library:
+        @staticmethod
+        def lin_prefill_workspace_size(_):
+            asked.append(at[0])
+            return 7
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", On)
+    monkeypatch.setattr(lin._lib, "load", lambda: Library)
+    args = lin._prefill_args(**_pre())
+    assert lin._prefill_workspace(args, 3) == lin._prefill_workspace(args, 0) == lin._prefill_workspace(args) == 7
+    assert asked == [3, 0, 0] and at == [0]
