@@ -201,7 +201,7 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
             if initial_state is None:
                 raise GDNError("with index, pass the pool as final_state or initial_state", 1)
             final_state = initial_state
-        elif v.dim() == 4 and q.dim() == 4:
+        elif v.dim() == 4 and q.dim() == 4 and (cu_seqlens is None or cu_seqlens.numel() > 1):
             rows = v.shape[0] if cu_seqlens is None else cu_seqlens.numel() - 1
             final_state = torch.empty((rows, v.shape[2], q.shape[3], v.shape[3]),
                                       dtype=torch.float32, device=q.device)

@@ -838,3 +838,10 @@ def test_states_of_one_layer_into_another(pkg):
     o = pkg.lin_decode(*token, want)
     assert torch.equal(pkg.lin_decode(*token, layers[:, 2], state_out=layers[:, 1], check=True), o)
     assert torch.equal(layers[:, 1], want) and torch.equal(layers[:, 2], S) and torch.equal(layers[:, 0], before[:, 0])
+
+
+def test_prefill_refuses_offsets_of_no_sequence(pkg):
+    q, k, v, g = (x.to(DEV) for x in make((1, 5), 1, 1, 64, 64, torch.bfloat16, 72))
+    for cu in (torch.empty(0), torch.zeros(1), torch.tensor(0)):
+        with pytest.raises(pkg.GDNError, match="cu_seqlens"):
+            pkg.lin_prefill(q, k, v, g, cu_seqlens=cu.to(torch.int32).to(DEV))
