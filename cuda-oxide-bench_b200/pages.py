@@ -82,7 +82,8 @@ def pages_copy(pools, src, dst, *, check: bool = False) -> None:
     Entries with a negative index are skipped.  So, with a device error, are
     entries whose index is out of range, whose destination another entry has
     too, or whose destination is some entry's source: what is copied does not
-    depend on the order of the copies."""
+    depend on the order of the copies.  An entry of a page onto itself moves
+    nothing and counts as neither."""
     pools, arr = _pools(pools)
     if not pools:
         raise GDNError("pages_copy needs a pool", 1)

@@ -484,7 +484,8 @@ size_t pages_workspace_size(const pages_args_t* args);
  * src or dst are skipped.  An entry is also skipped, with
  * GDN_DEVERR_BAD_INDEX, when an index is out of range, when another entry has
  * the same destination, or when its destination is some entry's source; so
- * what is copied does not depend on the order of the copies.  dst is read. */
+ * what is copied does not depend on the order of the copies.  An entry of a
+ * page onto itself moves nothing and counts as neither.  dst is read. */
 int pages_copy_launch(const pages_args_t* args, gdn_stream_t stream);
 
 /* dst[i] = the next free page, holding a copy of page src[i], i < n; the same

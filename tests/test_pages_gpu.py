@@ -250,3 +250,12 @@ def test_sources_just_behind_the_pool(pkg):
         for p in want:
             p[1], p[P - 1] = p[2], p[2]
         assert same(whole, want) and used.tolist() == [1] * P
+
+
+def test_copy_of_a_page_onto_itself_is_no_entry(pkg):
+    pools = make_pools(8, 9)
+    want = copies(pools)
+    for p in want:
+        p[5], p[1] = p[3].clone(), p[2].clone()
+    pkg.pages_copy(pools, i32([5, 3, 2, 2, 2]), i32([5, 5, 1, 2, 2]), check=True)
+    assert same(pools, want)
