@@ -61,4 +61,26 @@ int ensure_smem_attr(Kernel k, int bytes, std::atomic<uint64_t>& done_mask) {
   return GDN_OK;
 }
 
+// Launches a kernel that begins with pdl_launch_dependents() and pdl_wait(): it may
+// start while the kernel before it in the stream drains.
+template <typename... Args>
+int launch_pdl(void (*kern)(Args...), dim3 grid, unsigned threads, size_t smem, cudaStream_t stream,
+               const Args&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return GDN_ERR_LAUNCH;
+  }
+  return GDN_OK;
+}
+
 }  // namespace gdn

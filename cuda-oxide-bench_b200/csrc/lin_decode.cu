@@ -125,20 +125,8 @@ __global__ void __launch_bounds__(kThreads) lin_decode_kernel(const lin_decode_a
 
 template <int DK, int BV, typename IO>
 int launch(const lin_decode_args_t& a, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.Hv * (a.dv / BV)), static_cast<unsigned>(a.B < 65535 ? a.B : 65535));
-  cfg.blockDim = dim3(kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, lin_decode_kernel<DK, BV, IO>, a) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return GDN_ERR_LAUNCH;
-  }
-  return GDN_OK;
+  const dim3 grid(static_cast<unsigned>(a.Hv * (a.dv / BV)), static_cast<unsigned>(a.B < 65535 ? a.B : 65535));
+  return launch_pdl(lin_decode_kernel<DK, BV, IO>, grid, kThreads, 0, stream, a);
 }
 
 // The widest slab (at most 128 columns, and 128 registers of state a thread)

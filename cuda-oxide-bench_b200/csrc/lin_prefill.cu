@@ -1208,25 +1208,6 @@ int io_map(CUtensorMap* m, bool bf16, const void* base, int d, int heads, int T,
                     box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <typename... Args>
-int launch_pdl(void (*kern)(Args...), dim3 grid, int threads, int smem, cudaStream_t stream, const Args&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, args...) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return GDN_ERR_LAUNCH;
-  }
-  return GDN_OK;
-}
-
 // How the time axis is cut, and the workspace that takes.
 struct Cut {
   int piece = 0, pieces = 0;

@@ -283,25 +283,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
   }
 }
 
-template <typename Kernel, typename Arg>
-int launch_pdl(Kernel kern, unsigned grid, unsigned threads, size_t smem, cudaStream_t stream, const Arg& arg) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, arg) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return GDN_ERR_LAUNCH;
-  }
-  return GDN_OK;
-}
-
 bool small(const pages_args_t& a) { return a.pages <= kSmall && a.n <= kSmall; }
 
 // The pools, and the pieces of `most` pairs as a number of CTAs.

@@ -357,3 +357,16 @@ def test_workspace_is_asked_for_on_the_tensors_device(pkg, monkeypatch):
     args = lin._prefill_args(**_pre())
     assert lin._prefill_workspace(args, 3) == lin._prefill_workspace(args, 0) == lin._prefill_workspace(args) == 7
     assert asked == [3, 0, 0] and at == [0]
+
+
+def test_small_page_calls_need_no_workspace(pkg):
+    """What lets a call of few pages and entries go without asking for the size."""
+    small = graft.submodule("pages")._SMALL
+    L = pkg._lib.load()
+    for n in (1, small):
+        for pages in (1, small):
+            for remap in (0, BASE):
+                a = pages_args(pkg, pages=pages, n=n, remap=remap)
+                assert L.pages_workspace_size(ctypes.byref(a)) == 0
+    assert L.pages_workspace_size(ctypes.byref(pages_args(pkg, pages=1, n=small + 1, remap=0))) > 0
+    assert L.pages_workspace_size(ctypes.byref(pages_args(pkg, pages=small + 1, n=1))) > 0
