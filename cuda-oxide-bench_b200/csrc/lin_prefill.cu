@@ -26,8 +26,7 @@
 //   PV  O    += P V                then V applies the rows' factors and stages O
 // D0 and D1 lie between the others so that the tensor cores have work while R and
 // V prepare the next operand.  With f16 I/O QS, which R makes ready last, comes after
-// PV, and is three products: queries and state each in two parts of bf16, which has
-// the range for them, 2^-17 off.  All five take A from TMEM: a product with both
+// PV, and is a tf32 product: neither f16 nor, with as many bits, bf16 holds a state.  All five take A from TMEM: a product with both
 // operands in shared memory reads it at its full rate, and other warps' reads then
 // take five times as long (4 ldmatrix.x4: 726 cycles against 141).
 //
@@ -95,32 +94,30 @@ enum { kNear = 0, kNearBlock = 1, kFar = 2 };
 
 // TMEM columns; all 512 are allocated, so they start at 0
 constexpr uint32_t kTmSC = 0;     // scores fp32 [128]; P over its first 64 columns
-constexpr uint32_t kTmQLow = 64;  // f16: the lower part of Q' [DK / 2]
-constexpr uint32_t kTmQ = 128;    // Q, or Q' in bf16 [DK / 2]
+constexpr uint32_t kTmQ = 128;    // Q, or Q' in bf16 [DK / 2]; f16: Q' in tf32 [DK] up to kTmV
 constexpr uint32_t kTmV = 192;    // V'': lo [32], hi [32] of 64 tokens
 constexpr uint32_t kTmO = 256;    // O fp32 [BV]
 constexpr uint32_t kTmDS = 384;   // dS^T fp32 [DK]
 
 template <int DK, int BV, bool BF16, bool FULL>
 struct Layout {
-  // K and V in two stages; Q, which R takes into TMEM, in one, and K too where the two
-  // parts of S^T need its place
+  // K and V in two stages; Q, which R takes into TMEM, in one, and K too where a 32-bit
+  // S^T needs its place
   static constexpr int kKStages = !BF16 && FULL && DK == 128 && BV == 128 ? 1 : 2;
   static constexpr int kKTile = DK / 64 * kTile, kVTile = BV / 64 * kTile;
   static constexpr int kK = 0;
   static constexpr int kV = kKStages * kKTile;
   static constexpr int kQ = kV + 2 * kVTile;
-  static constexpr int kS = kQ + DK / 64 * kTile;          // S^T bf16 [BV][DK], 64-wide blocks; f16: high, low part
+  static constexpr int kS = kQ + DK / 64 * kTile;          // S^T bf16 [BV][DK], 64-wide blocks; f16: tf32, 32-wide ones
   static constexpr int kSBlock = BV * 128;
-  static constexpr int kSPart = DK / 64 * kSBlock;
-  static constexpr int kO = kS + (BF16 || !FULL ? 1 : 2) * kSPart;
+  static constexpr int kO = kS + (BF16 || !FULL ? DK / 64 : DK / 32) * kSBlock;
   static constexpr int kGate = kO + BV / 64 * kTile;
   static constexpr int kGateStage = 2 * kC * 4;            // G or its factors, w
   static constexpr int kFirst = kGate + 2 * kGateStage;    // per value column, a byte: see Bars::bad
   static constexpr int kShift = kFirst + 128;              // f16: x of V'' per value column, by chunk, a byte
   static constexpr int kRow = kShift + 2 * 128;            // f16: y of P per row, by chunk, a byte
   static constexpr int kBars = kRow + 2 * 128;
-  static constexpr int kBytes = kBars + 352;
+  static constexpr int kBytes = kBars + 360;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -134,6 +131,7 @@ struct Bars {
   uint64_t o_free, o_staged, o_stored, zeroed, drain;
   float gamma[2];
   float ref[2][4];  // R_b
+  int grow[2];      // f16: no G_i - G_j, i >= j, of the chunk is larger
   int form[2];      // kNear, kNearBlock, kFar
   // 1 + the last chunk in which dS is NaN; kFirst then holds, per value column, the first
   // token whose value is not finite (kC: none)
@@ -141,7 +139,7 @@ struct Bars {
   int call;         // the MMA thread to the rest of its warp
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 352, "barriers");
+static_assert(sizeof(Bars) <= 360, "barriers");
 
 struct PrefillParams {
   lin_prefill_args_t a;
@@ -503,9 +501,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       // below 2^-kLeast is taken as that; P carries the rest of it, and of the state
       // before the chunk so little arrives that it makes no difference.)  Else P carries
       // the row's factor, and QS takes Q' = scale e^G Q written over Q: in bf16, whose
-      // range it needs, and with f16 I/O in two parts of it, the lower one over the
-      // scores that P leaves free.  f16 does not have P's range either: both are taken
-      // times 2^-y, y by the row's largest of P, and the epilogue applies 2^y.
+      // range it needs, and with f16 I/O in tf32, in part over the scores that P leaves
+      // free; there the factor's power of two alone, which makes Q' exact, and the epilogue
+      // and P take the rest of it.  f16 does not have P's range either: both are taken
+      // times 2^-y, and the epilogue applies 2^y.  y comes from a bound of the row, its
+      // largest score by the scale and the gates' growth: P 2^-y stays below 2^15 and is
+      // lost 2^-39 below that, where the scores' fp32 sums are 2^-24 off.  (From P's own
+      // largest 208 us at B = 4, T = 4096, d = 128; this 190.)
       const bool by_block = BF16 && form == kNearBlock, plain_q = BF16 && form != kFar;
       const auto queries = [&](bool scaled) {
 #pragma unroll 1
@@ -514,18 +516,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             lds128(smem + L::kQ + b * kTile + tc::sw128_offset(row, e), &u[e >> 2][(e & 3) * 4]);
+          if (!BF16 && scaled) {
+#pragma unroll
+            for (int h4 = 0; h4 < 4; ++h4) {
+              uint32_t x[16];
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t w = u[h4 >> 1][(h4 & 1) * 8 + i];
+                x[2 * i] = __float_as_uint(f * tc::unpack_lo<BF16>(w));
+                x[2 * i + 1] = __float_as_uint(f * tc::unpack_hi<BF16>(w));
+              }
+              tc::tmem_st16(tmem + lanes + kTmV - DK + b * 64 + h4 * 16, x);
+            }
+            continue;
+          }
           if (scaled) {
 #pragma unroll
-            for (int h2 = 0; h2 < 2; ++h2) {
-              uint32_t lo[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                uint32_t& w = u[h2][i];
-                const float x = f * tc::unpack_lo<BF16>(w), y = f * tc::unpack_hi<BF16>(w);
-                w = tc::pack2<true>(x, y);
-                if (!BF16) lo[i] = tc::pack2<true>(x - tc::unpack_lo<true>(w), y - tc::unpack_hi<true>(w));
-              }
-              if (!BF16) tc::tmem_st16(tmem + lanes + kTmQLow + b * 32 + h2 * 16, lo);
+            for (int i = 0; i < 32; ++i) {
+              uint32_t& w = u[i >> 4][i & 15];
+              w = tc::pack2<true>(f * tc::unpack_lo<BF16>(w), f * tc::unpack_hi<BF16>(w));
             }
           }
           tc::tmem_st16(tmem + lanes + kTmQ + b * 32, u[0]);
@@ -549,67 +558,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!BF16 && (ok = wait(&bar.sc_done, c & 1))) tc::fence_after_sync();
       if (!ok) break;
-      // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16);
-      // in f16 a first round finds the row's largest
-      float most = 0.f, shrink = 1.f;
+      float shrink = 1.f, f_pow2 = 1.f;  // 2^-y, without the rest of f; f's power of two 2^-y
+      if (!BF16) {
+        float most = 0.f;
 #pragma unroll 1
-      for (int round = BF16; round < 2; ++round) {
+        for (int b = 0; b <= warp; b += 2) {
+          float x[4][16];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + e * 16, x[e]);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (e <= row - b * 32) most = fmaxf(most, fabsf(x[e >> 4][e & 15]));
+        }
+        const auto exponent = [](float x) { return static_cast<int>(__float_as_uint(fabsf(x)) >> 23) - 127; };
+        // y >= -64 and f 2^-y <= 2^91 keep Q' S and Q' within fp32; only rows of P that are
+        // zero come so low
+        const int y = max(max(exponent(most) + exponent(a.scale) + bar.grow[st] - 12, -64), exponent(f) - 90);
+        shrink = __uint_as_float(static_cast<uint32_t>(127 - min(y, 115)) << 23);
+        smem[L::kRow + st * 128 + row] = static_cast<unsigned char>(min(y, 115));
+        f_pow2 = shrink * __uint_as_float(__float_as_uint(f) & 0x7f800000u);
+        shrink *= __frcp_rn(tc::significand(f));
+      }
+      // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
 #pragma unroll 1
-        for (int b = 0; b < (round ? 4 : warp + 1); ++b) {
-          uint32_t u[16];
-          if (b <= warp) {
-            // the loads first: shared memory answers late while the products read it
-            float x[2][16], d[32];
-            tc::tmem_ld16(tmem + lanes + kTmSC + b * 32, x[0]);
-            tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
+      for (int b = 0; b < 4; ++b) {
+        uint32_t u[16];
+        if (b <= warp) {
+          // the loads first: shared memory answers late while the products read it
+          float x[2][16], d[32];
+          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32, x[0]);
+          tc::tmem_ld16(tmem + lanes + kTmSC + b * 32 + 16, x[1]);
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
-            if (form == kFar) {
+          for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
+          if (form == kFar) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
-            } else if (by_block) {
-              // the block's factor in two steps of at most 2^kSpan, or the row's as well
-              // (its root, twice: the whole may pass the range of a float where d is small)
-              const float r = ex2(0.5f * (Gi - fmaxf(Gi, -kLeast) - bar.ref[st][b]));
+            for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
+          } else if (by_block) {
+            // the block's factor in two steps of at most 2^kSpan, or the row's as well
+            // (its root, twice: the whole may pass the range of a float where d is small)
+            const float r = ex2(0.5f * (Gi - fmaxf(Gi, -kLeast) - bar.ref[st][b]));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
-            } else if (!BF16) {
-              const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
+            for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
+          } else if (!BF16) {
+            const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) d[e] *= r;
-            }
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] *= x[e >> 4][e & 15];
-            if (b == warp) {  // on the diagonal
-#pragma unroll
-              for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
-            }
-            if (!BF16) {
-              if (!round) {
-#pragma unroll
-                for (int e = 0; e < 32; ++e) most = fmaxf(most, fabsf(d[e]));
-                continue;
-              }
-#pragma unroll
-              for (int e = 0; e < 32; ++e) d[e] *= shrink;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = tc::pack2<BF16>(d[2 * e], d[2 * e + 1]);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = 0;
+            for (int e = 0; e < 32; ++e) d[e] *= r;
           }
-          tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
+          tc::tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) d[e] *= BF16 ? x[e >> 4][e & 15] : x[e >> 4][e & 15] * shrink;
+          if (b == warp) {  // on the diagonal
+#pragma unroll
+            for (int e = 0; e < 32; ++e) d[e] = e <= lane ? d[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = tc::pack2<BF16>(d[2 * e], d[2 * e + 1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 16; ++e) u[e] = 0;
         }
-        if (!round) {
-          // The row's largest of P 2^-y lies in [2^13, 2^14).  Q' S and Q' 2^-y bound y from
-          // below; for the second of them, only rows of P that are zero come so low.
-          const int y = max(max(static_cast<int>(__float_as_uint(most) >> 23) - 127 - 13, -64),
-                            static_cast<int>(__float_as_uint(fabsf(f)) >> 23) - 127 - 90);
-          shrink = __uint_as_float(static_cast<uint32_t>(127 - y) << 23);
-          smem[L::kRow + st * 128 + row] = static_cast<unsigned char>(y);
-        }
+        tc::tmem_st16(tmem + lanes + kTmSC + b * 16, u);
       }
       tc::tmem_wait_st();
       tc::fence_before_sync();
@@ -619,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&bar.gempty[st]);
       }
       if (!BF16) {
-        f *= shrink;
+        f = f_pow2;
         queries(true);
         tc::tmem_wait_st();
         tc::fence_before_sync();
@@ -732,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       if (!BF16) {
         const int y = static_cast<signed char>(smem[L::kRow + (c & 1) * 128 + row]);
-        factor = __uint_as_float(static_cast<uint32_t>(127 + y) << 23);
+        factor *= __uint_as_float(static_cast<uint32_t>(127 + y) << 23);
       }
 #pragma unroll 1
       for (int b = 0; b < BV / 32; ++b) {
@@ -805,12 +814,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after_sync();
         parts(c, half);
         if (half) {
-          if (FULL && BF16) {
+          if (FULL) {
             const float own = reinterpret_cast<const float*>(smem + L::kGate + st * L::kGateStage)[row];
             const int form = bar.form[st];
             factor = 1.f;
-            if (form == kNear) factor = a.scale * __frcp_rn(own);
-            if (form == kNearBlock) {
+            if (!BF16) {  // as R has it
+              const float Gi = form == kNearBlock ? bar.ref[st][quarter] - __log2f(own) : own;
+              factor = tc::significand(a.scale * (form == kNear ? __frcp_rn(own) : ex2(Gi)));
+            } else if (form == kNear) {
+              factor = a.scale * __frcp_rn(own);
+            } else if (form == kNearBlock) {
               const float Gi = bar.ref[st][quarter] + p.pow - __log2f(own);
               factor = p.rest * ex2(fmaxf(Gi, -kLeast));
             }
@@ -872,19 +885,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else if (c >= 0 && !(ok = wait(&bar.qs_done, c & 1))) {
         break;  // (in bf16 ds_done comes behind it)
       }
-      if (has_rows) {  // S^T rounded to bf16, the QS product's operand
+      if (has_rows && !BF16) {  // S^T rounded to tf32, the QS product's operand
+#pragma unroll
+        for (int i = 0; i < kN / 4; ++i) {
+          const int piece = half * (kN / 4) + i;
+          tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7), tc::to_tf32(S[4 * i]),
+                     tc::to_tf32(S[4 * i + 1]), tc::to_tf32(S[4 * i + 2]), tc::to_tf32(S[4 * i + 3]));
+        }
+      } else if (has_rows) {  // or to bf16
 #pragma unroll
         for (int i = 0; i < kN / 8; ++i) {
           const int piece = half * (kN / 8) + i;
-          if (!BF16) {  // the lower part; the upper one as in bf16
-            uint32_t lo[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t hi = tc::pack2<true>(S[8 * i + 2 * e], S[8 * i + 2 * e + 1]);
-              lo[e] = tc::pack2<true>(S[8 * i + 2 * e] - tc::unpack_lo<true>(hi), S[8 * i + 2 * e + 1] - tc::unpack_hi<true>(hi));
-            }
-            tc::sts128(sb + L::kS + L::kSPart + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7), lo[0], lo[1], lo[2], lo[3]);
-          }
           tc::sts128(sb + L::kS + (piece >> 3) * L::kSBlock + tc::sw128_offset(row, piece & 7),
                      tc::pack2<true>(m * S[8 * i], m * S[8 * i + 1]), tc::pack2<true>(m * S[8 * i + 2], m * S[8 * i + 3]),
                      tc::pack2<true>(m * S[8 * i + 4], m * S[8 * i + 5]), tc::pack2<true>(m * S[8 * i + 6], m * S[8 * i + 7]));
@@ -989,7 +1000,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         lo = fminf(lo, gv[e]);
         hi = fmaxf(hi, gv[e]);
       }
-      int form = kNear;
+      int form = kNear, grow = 0;
       float ref = 0.f;  // kNearBlock: R of this lane's block (8 lanes)
       if (FULL) {
 #pragma unroll
@@ -1007,6 +1018,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float end_of_block = __shfl_sync(0xffffffffu, gv[3], lane | 7);
         form = lo >= -kLeast && hi <= kMost ? kNear : near_block ? kNearBlock : kFar;
         if (form == kNearBlock) ref = end_of_block;
+        const bool rises = x[0] > 0.f || x[1] > 0.f || x[2] > 0.f || x[3] > 0.f;
+        if (!BF16 && __any_sync(0xffffffffu, rises)) {
+          float low = fminf(fminf(gv[0], gv[1]), fminf(gv[2], gv[3])), up = 0.f;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const float y = __shfl_up_sync(0xffffffffu, low, off);
+            if (lane >= off) low = fminf(low, y);
+          }
+          low = __shfl_up_sync(0xffffffffu, low, 1);
+          if (lane == 0) low = gv[0];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            low = fminf(low, gv[e]);
+            up = fmaxf(up, gv[e] - low);
+          }
+          grow = __reduce_max_sync(0xffffffffu, __float2int_ru(fminf(up, 200.f)));
+        }
         if (form != kFar) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) gv[e] = ex2(ref - gv[e] + (BF16 ? p.pow : 0.f));
@@ -1028,6 +1056,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         bar.gamma[st] = ex2(end);
         bar.form[st] = form;
+        if (FULL && !BF16) bar.grow[st] = grow;
       }
       if (FULL && (lane & 7) == 7) bar.ref[st][lane >> 3] = ref;
       __syncwarp();
@@ -1123,15 +1152,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int s = 0; s < kC / 16; ++s)
           tc::mma_tmem_a(kTmO, kTmSC + s * 8, v + s * 128, kIdPV, BF16 || s > 0);
         tc::commit(&bar.empty[kTileV][st]);
-        if constexpr (!BF16) {  // lower part of Q', lower part of S^T, the upper ones
+        if constexpr (!BF16) {
           if (!(ok = wait1(&bar.q2_ready, c & 1, &bar.s_ready, c & 1, &bar.s_ready, c & 1))) break;
           tc::fence_after_sync();
 #pragma unroll
-          for (int part = 0; part < 3; ++part)
-#pragma unroll
-            for (int s = 0; s < DK / 16; ++s)
-              tc::mma_tmem_a(kTmO, (part ? kTmQ : kTmQLow) + s * 8, sT + along(s, L::kSBlock) + (part == 1 ? L::kSPart >> 4 : 0),
-                             kIdQS, true);
+          for (int s = 0; s < DK / 8; ++s)
+            tc::mma_tmem_a_tf32(kTmO, kTmV - DK + s * 8, sT + along(s, L::kSBlock), tc::idesc_tf32(128, BV), true);
           tc::commit(&bar.qs_done);
         }
         tc::commit(&bar.pv_done);

@@ -57,6 +57,11 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool a_mn, bool b
          | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
 }
 
+// The same for tf32 inputs (32 bits each, of which the lowest 13 are not used), both K-major.
+__host__ __device__ constexpr uint32_t idesc_tf32(int M, int N) {
+  return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
 // ---------------------------------------------------------------- MMA
 __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t idesc,
                                     bool accumulate) {
@@ -162,6 +167,17 @@ __device__ __forceinline__ void mma_tmem_a(uint32_t d_tmem, uint32_t a_tmem, uin
       : "memory");
 }
 
+// The same with tf32 inputs: 8 of them per step, one per 32-bit column.
+__device__ __forceinline__ void mma_tmem_a_tf32(uint32_t d_tmem, uint32_t a_tmem, uint64_t b,
+                                                uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(accumulate))
+      : "memory");
+}
+
 // True in one lane of a converged warp.  The compiler knows the instruction: in
 // code under it, tcgen05 and TMA operands go straight to uniform registers, where
 // under a test of the lane number each issue carries a sequence for many lanes.
@@ -216,6 +232,18 @@ __device__ __forceinline__ uint32_t bf16_rne_bits(float x) {
 // The float value of x rounded to bf16.
 __device__ __forceinline__ float bf16_round(float x) {
   return __uint_as_float(bf16_rne_bits(x) & 0xFFFF0000u);
+}
+
+// x rounded to tf32 (11 significant bits, the range of fp32).
+__device__ __forceinline__ uint32_t to_tf32(float x) {
+  uint32_t u;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(u) : "f"(x));
+  return u;
+}
+// x over the power of two that is its exponent (of zero and smaller than normal numbers: as
+// if they were 2^0): +-[1, 2).
+__device__ __forceinline__ float significand(float x) {
+  return __uint_as_float((__float_as_uint(x) & 0x807fffffu) | 0x3f800000u);
 }
 
 // packs two floats into a bf16x2 / f16x2 word (low half = first)

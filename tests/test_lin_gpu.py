@@ -706,8 +706,8 @@ def test_prefill_f16_growing_gates_keep_the_state(pkg):
 
 
 def check_f16_rows(o, ref, v):
-    """f16 I/O: the output's rounding and that of P (u each of its terms; numbers below 2^-14 by at most 2^-25),
-    queries and states in two parts of bf16 (each 2^-18, the product of the lower parts as much)."""
+    """f16 I/O: the output's rounding, and that of P or of the state that the queries meet, tf32 (u each, of their
+    terms); a scaled P below 2^-14 is off by at most 2^-25 (of the unscaled, a little more: hence 2^-16)."""
     ro, _, oa, _ = ref
     u = half_step(torch.float16)
     tol = u * ro.abs() + 2.0 ** -25 + (u + 2.0 ** -16 + 64 * E) * oa + 2.0 ** -25 * 128 * v.double().abs().amax()
@@ -845,3 +845,16 @@ def test_prefill_refuses_offsets_of_no_sequence(pkg):
     for cu in (torch.empty(0), torch.zeros(1), torch.tensor(0)):
         with pytest.raises(pkg.GDNError, match="cu_seqlens"):
             pkg.lin_prefill(q, k, v, g, cu_seqlens=cu.to(torch.int32).to(DEV))
+
+
+@pytest.mark.parametrize("rise", [0.01, 3.0])
+@pytest.mark.parametrize("gmin", [-0.5, -2.0, -30.0])
+def test_prefill_f16_a_gate_that_grows_among_falling_ones(pkg, gmin, rise):
+    T, d, io = 200, 64, torch.float16
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 73, gmin=gmin)
+    g[0, [3, 70, 71, 127, 190]] = rise
+    S0 = torch.randn(1, 2, d, d, generator=torch.Generator().manual_seed(74))
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=0.1, check=True)
+    ref = steps(q[0], k[0], v[0], g[0], S0[0], 0.1)
+    check_f16_rows(o[0].cpu(), ref, v)
+    check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0], v[0])
