@@ -397,14 +397,20 @@ __device__ __noinline__ void clear_values(unsigned char* tile, int columns, uint
   for (int x = (threadIdx.x & 31) * 2; x < columns; x += 64) {
     unsigned char* at = tile + (x >> 6) * kTile + (x & 7) * 2;
     int first0 = kC, first1 = kC;
-#pragma unroll 4
-    for (int t = kC - 1; t >= 0; --t) {
-      uint32_t* v = reinterpret_cast<uint32_t*>(at + tc::sw128_offset(t, (x & 63) >> 3));
-      const uint32_t u = *v;
-      const bool bad0 = (u & exponent) == exponent, bad1 = (u >> 16 & exponent) == exponent;
-      if (bad0) first0 = t;
-      if (bad1) first1 = t;
-      if (bad0 || bad1) *v = (bad0 ? 0u : u & 0xffffu) | (bad1 ? 0u : u & 0xffff0000u);
+#pragma unroll 1
+    for (int t0 = kC - 8; t0 >= 0; t0 -= 8) {  // rows of one swizzle atom, loads first
+      uint32_t u[8];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) u[t] = *reinterpret_cast<uint32_t*>(at + tc::sw128_offset(t0 + t, (x & 63) >> 3));
+#pragma unroll
+      for (int t = 7; t >= 0; --t) {
+        const bool bad0 = (u[t] & exponent) == exponent, bad1 = (u[t] >> 16 & exponent) == exponent;
+        if (bad0) first0 = t0 + t;
+        if (bad1) first1 = t0 + t;
+        if (bad0 || bad1)
+          *reinterpret_cast<uint32_t*>(at + tc::sw128_offset(t0 + t, (x & 63) >> 3)) =
+              (bad0 ? 0u : u[t] & 0xffffu) | (bad1 ? 0u : u[t] & 0xffff0000u);
+      }
     }
     first[x] = static_cast<unsigned char>(first0);
     first[x + 1] = static_cast<unsigned char>(first1);
@@ -417,9 +423,13 @@ __device__ __noinline__ void clear_values(unsigned char* tile, int columns, uint
 // or one before belongs to which is not finite.
 __device__ __noinline__ void mark_row(unsigned char* tile, int row, int columns, const unsigned char* first) {
 #pragma unroll 1
-  for (int x = 0; x < columns; ++x)
-    if (row >= first[x])
-      *reinterpret_cast<uint16_t*>(tile + (x >> 6) * kTile + tc::sw128_offset(row, (x & 63) >> 3) + (x & 7) * 2) = 0x7fff;
+  for (int x0 = 0; x0 < columns; x0 += 8) {
+    const uint2 f = *reinterpret_cast<const uint2*>(first + x0);
+    uint16_t* o = reinterpret_cast<uint16_t*>(tile + (x0 >> 6) * kTile + tc::sw128_offset(row, (x0 & 63) >> 3));
+#pragma unroll
+    for (int x = 0; x < 8; ++x)
+      if (row >= static_cast<int>((x < 4 ? f.x : f.y) >> (x & 3) * 8 & 0xffu)) o[x] = 0x7fff;
+  }
 }
 
 // FULL: everything.  Else only what a piece adds to the state and its decay, from k,
