@@ -11,8 +11,9 @@
 // side.  So there is no ring and no producer warp: a CTA takes one DK x BV slab of
 // a head's state (columns are independent), every thread issues the loads of all
 // its rows at once, and the CTAs resident on an SM hide each other's latency.
-// B = 1024, H = 32, d = 128: 641 us, 6.7 TB/s of state, the measured copy's rate and
-// what the GDN decode's ring reaches; with pages in random order 5% less.
+// B = 1024, H = 32, d = 128: 647 to 662 us, 6.5 to 6.7 TB/s of state, the measured copy's
+// rate and what the GDN decode's ring reaches; with pages in random order 5% less.  d =
+// 256 x 128, B = 512: 723 to 730 us, 0.91 of that rate.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -21,8 +22,8 @@
 namespace gdn {
 namespace {
 
-// 128 threads: at B = 1024, H = 32, d = 128 a 128-column slab takes 641 us (6.70 TB/s
-// of state) with 128 threads, 972 with 256 and 996 with 512.  More threads per slab
+// 128 threads: at B = 1024, H = 32, d = 128, in bursts, a 128-column slab takes 641 us
+// (6.70 TB/s of state) with 128 threads, 972 with 256 and 996 with 512.  More threads per slab
 // mean fewer slabs on an SM, whose loads, arithmetic and stores then overlap less.
 constexpr int kThreads = 128;
 

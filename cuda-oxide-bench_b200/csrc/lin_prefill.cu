@@ -25,20 +25,28 @@
 //   D1  dS^T += V''^T K            of the others; then S reads dS and rewrites S^T
 //   PV  O    += P V                then V applies the rows' factors and stages O
 // D0 and D1 lie between the others so that the tensor cores have work while R and
-// V prepare the next operand.  With f16 I/O QS, which R makes ready last, comes after
-// PV, and is a tf32 product: neither f16 nor, with as many bits, bf16 holds a state.  All five take A from TMEM: a product with both
+// V prepare the next operand.  All five take A from TMEM: a product with both
 // operands in shared memory reads it at its full rate, and other warps' reads then
 // take five times as long (4 ldmatrix.x4: 726 cycles against 141).
 //
 // V'' = w v, w = e^(G_C - G_j), is split into two parts of the I/O type, hi +
-// lo, because the state is kept to fp32 accuracy: one part would leave half a
-// step of the I/O type of every term (2^-8 in bf16).  In bf16 so is w, which makes
-// both parts a few packed fused multiply-adds: hi = v w_hi + v w_lo rounded once, lo =
-// (v w_hi - hi) + v w_lo, the difference being exact.  f16 has the range for neither:
-// there w v is formed in fp32 and split times 2^-x, x by the largest of its value
-// column, so that a part is lost only 2^-39 below that; S applies 2^x to dS.  Against
-// 64 bits the state is off by 3e-6, the bf16 output by 2.4e-3 (1.7e-3 of it its own rounding; P and the
-// state that QS takes, each rounded to bf16 once, give the rest).
+// lo: one part would leave half a step of the I/O type of every term (2^-8 in bf16) in a
+// state that is fp32.  In bf16 so is w, which makes both parts a few packed fused
+// multiply-adds: hi = v w_hi + v w_lo rounded once, lo = (v w_hi - hi) + v w_lo, the
+// difference being exact.  Two parts of bf16 have 16 bits, and the state is off by up to
+// 3.4e-6 of its norm; a third part, which would make that 2e-8, takes 14 instructions a
+// pair of values in place of 5 and columns of TMEM that are all taken at d = 128.
+//
+// bf16 outputs are off by 2.4e-3: 1.7e-3 is their own rounding, P and the state that QS
+// takes, each rounded to bf16 once as the operands that they are, give the rest.
+//
+// f16 I/O: w v, P and the state have no place in f16's range, and less than its precision
+// in one part of bf16.  So w v is formed in fp32 and split times 2^-x, x by the largest of
+// its value column (a part is lost only 2^-39 below that; the state is off by 2e-7); P is
+// taken times 2^-y, y by its row; and QS, which R makes ready last and which then comes
+// after PV, is a tf32 product, with 11 bits as f16 but fp32's range.  Outputs are off by
+// 2.9e-4, 2.1e-4 of it their own rounding.  That costs V and R: at the shape below 185 to
+// 200 us in bursts against bf16's 99 to 103.
 //
 // A value of V that is not finite belongs to the rows from its own on, but P V would
 // bring it to the earlier ones of its chunk, as 0 x NaN.  It makes its column's dS NaN
@@ -46,14 +54,14 @@
 // place in the tile, and the epilogue writes NaN into its column from its row on.  (4% of
 // the time, at d = 64 9%; a test of each value by V took 6% and 14%.)
 //
-// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 115 to 120 us, 403 MB,
-// so 3.4 TB/s or 0.52 of the measured copy; 97 us in a burst, before the power limit
-// takes the clock to 1.6 GHz): a CTA takes 4700 cycles a chunk.  The products take 0.54
-// of them, and shared memory is at work in most: operands 1280 cycles of 128 bytes, TMA
-// 1000, the warps' reads, writes and barriers 2100.  Each answer from it takes some 250
+// What bounds it (B = 4, T = 4096, Hqk = 16, H = 32, d = 128, bf16: 118 to 126 us, 403 MB,
+// so 3.3 TB/s or 0.5 of the measured copy; 99 to 103 us in a burst, before the power limit
+// takes the clock to 1.6 GHz): a CTA takes 4550 cycles a chunk.  The products take 0.49
+// of them, and shared memory is at work in 0.92: operands 1280 cycles of 128 bytes, TMA
+// 1000, the warps' reads, writes and barriers 1900.  Each answer from it takes some 250
 // cycles then, in the chain Q, SC, P, PV of a chunk.  And instruction fetch: five
 // roles of straight-line code pass through the SM's instruction cache once a chunk, at
-// 0.92 hits.  So loops are kept rolled and call sites single where that is possible;
+// 0.89 hits.  So loops are kept rolled and call sites single where that is possible;
 // unrolled throughout, the same kernel took 226 us.
 #include <cuda_runtime.h>
 
@@ -73,8 +81,9 @@ constexpr int kThreads = 20 * 32;
 constexpr int kWarpV = 4, kWarpS = 8, kWarpTma = 16, kWarpGate = 17, kWarpMma = 18, kWarpStore = 19;
 constexpr float kLog2e = 1.4426950408889634f;
 // Up to so many sequences of a packed batch are put in order of length: 24 ragged ones
-// take 89.6 us and not 98, 32 of 20000 tokens 192 and not 203; 200, whose order takes
-// each of 3200 CTAs 2 us to find, 409 and not 365.
+// (f16, d = 128 x 64, before its parts cost what they do now) took 89.6 us and not 98, 32
+// of 20000 tokens 192 and not 203; 200, whose order takes each of 3200 CTAs 2 us to find,
+// 409 and not 365.
 constexpr int kRanked = 64;
 // log2 gates are cut off here: 2^-160 is zero in fp32, and cumulative sums stay finite
 constexpr float kLowest = -160.f;
@@ -517,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // times 2^-y, and the epilogue applies 2^y.  y comes from a bound of the row, its
       // largest score by the scale and the gates' growth: P 2^-y stays below 2^15 and is
       // lost 2^-39 below that, where the scores' fp32 sums are 2^-24 off.  (From P's own
-      // largest 208 us at B = 4, T = 4096, d = 128; this 190.)
+      // largest 105 us at B = 4, T = 2048, d = 128; this 99.)
       const bool by_block = BF16 && form == kNearBlock, plain_q = BF16 && form != kFar;
       const auto queries = [&](bool scaled) {
 #pragma unroll 1
@@ -1267,10 +1276,11 @@ Cut choose_cut(const lin_prefill_args_t& a, int sms) {
     cut.slots = 2 * (static_cast<int64_t>(a.T) / cut.piece);
   } else {
     // Cost in chunks of time (2.5 us), kStart of them to start a CTA, a piece's state
-    // pass kState of a whole one, kScan for the scan and the launches.  Measured, d =
-    // 128, one sequence: 32 heads, 32768 tokens 700 us whole, 317 in 9 pieces (345 in
-    // 4, 401 in 7); 8 heads 95 in 18 (146 in 9); 32 heads, 4096 tokens 55 in 4 (70 in 9);
-    // two sequences of 8192 (64 CTAs) 172 to 185 in 2 and 190 in 4.
+    // pass kState of a whole one, kScan for the scan and the launches.  Measured in bursts
+    // (a call among others 10% more), d = 128, one sequence: 32 heads, 32768 tokens 700 us
+    // whole, 317 in 9 pieces (345 in 4, 401 in 7); 8 heads 95 in 18 (146 in 9); 32 heads,
+    // 4096 tokens 55 in 4 (70 in 9); two sequences of 8192 (64 CTAs) 172 to 185 in 2 and
+    // 190 in 4.
     constexpr double kStart = 2.0, kState = 0.5, kScan = 3.0;
     const auto waves = [&](int64_t ctas) { return static_cast<double>((ctas + sms - 1) / sms); };
     double best = 0.95 * waves(rows * a.B) * (chunks + kStart);

@@ -174,7 +174,8 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
 
     ``cu_seqlens`` (int32 [N + 1] on the device) packs N sequences end to end
     into a batch of one; sequence n is rows cu_seqlens[n] .. cu_seqlens[n+1] - 1,
-    possibly none, and rows outside every sequence are left as they were.
+    possibly none, and rows outside every sequence are left as they were (T, all
+    rows, is at least 1).
 
     With ``index`` (int32 on the device, one entry per sequence) the states are
     pools: sequence n starts from page index[n] of ``initial_state`` and leaves
@@ -187,11 +188,13 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
 
     Few heads and a long T: the time axis is cut, with a workspace from torch's
     allocator (or ``workspace``, at least as large).  Infinities and NaN in a row
-    reach no earlier row and no other sequence; outputs that a value of v which is
-    not finite belongs to are NaN within its chunk.  f16: P = q.k e^(G_i - G_j) scale and e^(G_C - G_j) v
-    have to stay below 65504, which only large values or growing gates pass. bf16:
-    under strong decay outputs hold up to 2^47, and a row keeps 2^-80 of the state
-    before its chunk where the decay would leave less.
+    reach no earlier row and no other sequence; the outputs they belong to are not
+    finite.  bf16: the decayed scores, and the state where the queries meet it, are
+    rounded to bf16 once, the state itself takes its terms in 16 bits; under strong
+    decay outputs hold up to 2^47, and a row keeps 2^-80 of the state before its chunk
+    (128 tokens) where the decay would leave less.  f16: scores rounded to f16 times a
+    power of two of their row, the state where the queries meet it to tf32, its terms
+    in 22 bits; scores and states may pass f16's range (about twice the time of bf16).
     """
     dev = _on(q, k, v, g, initial_state, final_state, out, cu_seqlens, index, workspace)
     if out is None:

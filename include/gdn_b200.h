@@ -364,9 +364,9 @@ int gdn_gather_wait_counter(const uint32_t* counter, uint32_t target, uint32_t* 
  *
  * with a_t = exp(g_t) a scalar per value head, data-dependent (g per token)
  * or fixed (one g per head; strides of 0 over batch and time).  Heads, the
- * state layout and q/k head sharing are those of the gated delta rule.  The
- * reference has no such operator; layers of this kind alternate with GDN
- * layers in hybrid models and keep the same states.
+ * state layout and q/k head sharing are those of the gated delta rule, so a
+ * cache may hold the states of layers of both kinds.  The reference has no
+ * such operator.
  *
  * States may live in a pool of pages [P, Hv, d_k, d_v], one page per sequence
  * (page p at state + p * state_sp elements; contiguous inside).  With `index`
@@ -379,8 +379,10 @@ int gdn_gather_wait_counter(const uint32_t* counter, uint32_t target, uint32_t* 
  * One token per sequence.  A row without a page gets a zero output row and
  * touches no state.  Strides are in ELEMENTS; rows of q/k/v/o are contiguous,
  * their bases and strides 16-byte aligned, as are the states (state_sp a
- * multiple of 4).  state_out may equal state_in (in place) or be disjoint
- * from it; the pages of idle rows are not copied to a disjoint state_out.
+ * multiple of 4); the stride of an axis of one entry is not looked at.
+ * state_out may equal state_in (in place) or be disjoint from it, also with its
+ * pages between state_in's (layers of one tensor); the pages of idle rows are
+ * not copied to a disjoint state_out.
  * d_k in {64, 128, 256}, d_v a multiple of 64.
  */
 typedef struct {
@@ -417,10 +419,20 @@ int lin_decode_launch(const lin_decode_args_t* args, gdn_stream_t stream);
  * state in the same page of final_state, which may equal initial_state or be
  * disjoint from it.  A sequence with a negative index starts from zero and
  * its state is not kept; one of no tokens keeps its initial state.
- * d_k in {64, 128}, d_v a multiple of 64.  Strides as for the decode step, and
- * positive on every axis of more than one entry (g's may be 0).  o must not
- * share memory with q, k or v.  Log gates only.  Workspace: lin_prefill_workspace_size(args) bytes (0 for
- * many shapes), 16-byte aligned, owned by the caller.
+ * d_k in {64, 128}, d_v a multiple of 64, T at least 1.  Strides as for the
+ * decode step, and positive on every axis of more than one entry (g's may be
+ * 0).  o must not share memory with q, k or v.  Log gates only.  Workspace:
+ * lin_prefill_workspace_size(args) bytes (0 for many shapes), 16-byte aligned,
+ * owned by the caller.
+ *
+ * Numbers.  A value that is not finite reaches no row before its own and no
+ * other sequence; the outputs it belongs to are not finite.  bf16 I/O: the decayed
+ * scores, and the state where the queries meet it, are rounded to bf16 once; the
+ * state itself takes its terms in 16 bits and sums in fp32; outputs hold up to
+ * 2^47, and a row takes 2^-80 of the state before its 128-token chunk where the
+ * decay would leave less.  f16 I/O: the decayed scores are rounded to f16 times a
+ * power of two of their row, the state where the queries meet it to tf32; the
+ * state itself takes its terms in 22 bits; scores and states may pass f16's range.
  */
 typedef struct {
   const void* q;              /* [B, T, Hqk, d_k] or packed [T, Hqk, d_k]    */
