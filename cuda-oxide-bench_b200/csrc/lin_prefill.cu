@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!BF16 && (ok = wait(&bar.sc_done, c & 1))) tc::fence_after_sync();
       if (!ok) break;
-      float shrink = 1.f, f_pow2 = 1.f;  // 2^-y, without the rest of f; f's power of two 2^-y
+      float shrink = 1.f, f_pow2 = 1.f;  // scale 2^-y, without the rest of f; f's power of two 2^-y
       if (!BF16) {
         float most = 0.f;
 #pragma unroll 1
@@ -591,13 +591,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (e <= row - b * 32) most = fmaxf(most, fabsf(x[e >> 4][e & 15]));
         }
         const auto exponent = [](float x) { return static_cast<int>(__float_as_uint(fabsf(x)) >> 23) - 127; };
-        // y >= -64 and f 2^-y <= 2^91 keep Q' S and Q' within fp32; only rows of P that are
-        // zero come so low
-        const int y = max(max(exponent(most) + exponent(a.scale) + bar.grow[st] - 12, -64), exponent(f) - 90);
+        // (a score that is not zero is 2^-48 at least.)  y >= -64 and f 2^-y <= 2^91 keep Q' S
+        // and Q' within fp32; only rows of P that are zero come so low
+        const int y = max(max(max(exponent(most), -48) + exponent(a.scale) + bar.grow[st] - 12, -64), exponent(f) - 90);
         shrink = __uint_as_float(static_cast<uint32_t>(127 - min(y, 115)) << 23);
         smem[L::kRow + st * 128 + row] = static_cast<unsigned char>(min(y, 115));
         f_pow2 = shrink * __uint_as_float(__float_as_uint(f) & 0x7f800000u);
-        shrink *= __frcp_rn(tc::significand(f));
+        shrink *= a.scale * __frcp_rn(tc::significand(f));
       }
       // P in the I/O type over the scores: columns [32 b, 32 b + 32) go to [16 b, 16 b + 16)
 #pragma unroll 1
@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int e = 0; e < 32; e += 4) lds128(G + b * 32 + e, d + e);
           if (form == kFar) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) d[e] = a.scale * ex2(Gi - d[e]);
+            for (int e = 0; e < 32; ++e) d[e] = (BF16 ? a.scale : 1.f) * ex2(Gi - d[e]);
           } else if (by_block) {
             // the block's factor in two steps of at most 2^kSpan, or the row's as well
             // (its root, twice: the whole may pass the range of a float where d is small)
@@ -620,7 +620,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] = d[e] * r * r;
           } else if (!BF16) {
-            const float r = form == kNear ? f : a.scale * ex2(Gi - bar.ref[st][b]);
+            const float r = form == kNear ? __frcp_rn(own) : ex2(Gi - bar.ref[st][b]);
 #pragma unroll
             for (int e = 0; e < 32; ++e) d[e] *= r;
           }

@@ -858,3 +858,23 @@ def test_prefill_f16_a_gate_that_grows_among_falling_ones(pkg, gmin, rise):
     ref = steps(q[0], k[0], v[0], g[0], S0[0], 0.1)
     check_f16_rows(o[0].cpu(), ref, v)
     check_prefill(o[0].cpu(), S[0].cpu(), ref, io, k[0], v[0])
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gmin", [-0.5, -1.5, -3.0, -30.0])
+def test_prefill_keys_of_zero_at_a_large_scale(pkg, gmin, io):
+    """No decay times the scale may pass fp32 on the way to a product with zero."""
+    T, d, scale = 140, 64, 2.0 ** 100
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 75, gmin=gmin)
+    k[:] = 0
+    S0 = torch.randn(1, 2, d, d, generator=torch.Generator().manual_seed(76)) / scale
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), scale=scale, check=True)
+    ro, _, oa, _ = steps(q[0], k[0], v[0], g[0], S0[0], scale)
+    u = half_step(io)
+    # a row takes 2^-80 of the state before its chunk where decay leaves less
+    at = scale * torch.einsum("td,hde->the", q[0, :, 0].double().abs(), S0[0].double().abs())
+    # the state itself, of 2^-100 and decaying, comes below fp32's smallest normal number, where its steps are 2^-149
+    # wide: each of its entries may be off by one, and scale |q| of them make the output
+    at += scale * 2.0 ** (80 - 149) * q[0].double().abs().sum(-1, keepdim=True)
+    tol = u * ro.abs() + (u + 2 * W + 64 * E) * oa + 2.0 ** -80 * at + (2.0 ** -25 if io == torch.float16 else 2.0 ** -126)
+    assert bool(((o[0].cpu().double() - ro).abs() <= tol).all())
