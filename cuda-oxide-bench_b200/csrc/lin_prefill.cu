@@ -126,7 +126,7 @@ struct Layout {
   static constexpr int kShift = kFirst + 128;              // f16: x of V'' per value column, by chunk, a byte
   static constexpr int kRow = kShift + 2 * 128;            // f16: y of P per row, by chunk, a byte
   static constexpr int kBars = kRow + 2 * 128;
-  static constexpr int kBytes = kBars + 360;
+  static constexpr int kBytes = kBars + 368;
   static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -136,7 +136,7 @@ struct Bars {
   uint64_t full[3][2], empty[3][2];  // of the Q (one stage), K, V tiles
   uint64_t gfull[2], gempty[2];
   uint64_t sc_done, q_ready, q2_ready, qs_done, p_ready, pv_done;
-  uint64_t v_ready[2], v_free[2], ds_done, ds_free, s_ready;
+  uint64_t v_ready[2], v_free[2], ds_done, seen, ds_free, s_ready;
   uint64_t o_free, o_staged, o_stored, zeroed, drain;
   float gamma[2];
   float ref[2][4];  // R_b
@@ -148,7 +148,7 @@ struct Bars {
   int call;         // the MMA thread to the rest of its warp
   uint32_t tmem;
 };
-static_assert(sizeof(Bars) <= 360, "barriers");
+static_assert(sizeof(Bars) <= 368, "barriers");
 
 struct PrefillParams {
   lin_prefill_args_t a;
@@ -471,6 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&bar.q_ready, 4);
     mbar_init(&bar.q2_ready, 4);
     mbar_init(&bar.ds_free, 8);
+    mbar_init(&bar.seen, 8);
     mbar_init(&bar.qs_done, 1);
     mbar_init(&bar.p_ready, 4);
     mbar_init(&bar.pv_done, FULL ? 2 : 1);
@@ -718,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const auto parts = [&](int c, int half) {
       const int st = c & 1;
       if (has_rows) {
-        if (!BF16 && !half) find_shifts(st);
+        if (!BF16 && !FULL && !half) find_shifts(st);
         uint32_t ww[4][4], r[2][4][4];
         weights(st, half, ww);
         // all loads first (unrolled 98.2 against 99.5 us; at d = 64 37.9 against 40.7)
@@ -827,6 +828,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!(ok = wait(&bar.zeroed, 0))) break;  // only the last chunk is short
           }
         }
+        // meanwhile (S has read the shifts of the chunk before last: D0 of the last waited for it)
+        if (!BF16 && FULL && !half && has_rows) find_shifts(st);
         // the columns' last user: the half before, or this half of the chunk before
         const int before = FULL ? step - 1 : step - 2;
         if (before >= 0 && !(ok = wait(&bar.v_free[before & 1], (before >> 1) & 1))) break;
@@ -877,17 +880,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (has_rows) {
           const int x = BF16 ? 0 : static_cast<signed char>(smem[L::kShift + st * 128 + row]);
           const float grow = __uint_as_float(static_cast<uint32_t>(127 + x) << 23);
-          bool bad = false;
 #pragma unroll
           for (int b = 0; b < kN / 16; ++b) {
             float d[16];
             tc::tmem_ld16(tmem + lanes + kTmDS + half * kN + b * 16, d);
             tc::tmem_wait_ld();
-            if (b == 0) bad = isnan(d[0]);
+            if (FULL && b == 0) {  // at once: PV waits for it
+              const bool bad = __any_sync(0xffffffffu, isnan(d[0]));
+              if (lane == 0) {
+                if (bad) bar.bad = c + 1;
+                mbar_arrive(&bar.seen);
+              }
+            }
 #pragma unroll
             for (int e = 0; e < 16; ++e) S[b * 16 + e] = fmaf(gamma, S[b * 16 + e], BF16 ? d[e] : grow * d[e]);
           }
-          if (FULL && __any_sync(0xffffffffu, bad) && lane == 0) bar.bad = c + 1;
+        } else if (FULL && lane == 0) {
+          mbar_arrive(&bar.seen);
         }
         tc::fence_before_sync();
         __syncwarp();
@@ -1159,7 +1168,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc::commit(&bar.empty[kTileK][kst]);
 
       if constexpr (FULL) {
-        ok = wait1(&bar.p_ready, c & 1, &bar.ds_free, c & 1, BF16 ? &bar.p_ready : &bar.o_free, BF16 ? c & 1 : (c & 1) ^ 1);
+        // seen: bar.bad says whether V holds only finite values
+        ok = wait1(&bar.p_ready, c & 1, &bar.seen, c & 1, BF16 ? &bar.p_ready : &bar.o_free, BF16 ? c & 1 : (c & 1) ^ 1);
         if (!ok) break;
         if (*static_cast<volatile int*>(&bar.bad) == c + 1) {
           bar.call = c + 1;
