@@ -878,3 +878,57 @@ def test_prefill_keys_of_zero_at_a_large_scale(pkg, gmin, io):
     at += scale * 2.0 ** (80 - 149) * q[0].double().abs().sum(-1, keepdim=True)
     tol = u * ro.abs() + (u + 2 * W + 64 * E) * oa + 2.0 ** -80 * at + (2.0 ** -25 if io == torch.float16 else 2.0 ** -126)
     assert bool(((o[0].cpu().double() - ro).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+def test_prefill_packed_long_pages_and_values_that_are_not_finite(pkg, io):
+    """Cut and whole sequences side by side, some of them with values that are not finite: those stay where they are."""
+    Hv, dk, dv = 2, 128, 128
+    lens = [100, 9000, 0, 2049, 300, 1]
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    q, k, v, g = make((1, cu[-1]), 1, Hv, dk, dv, io, 77, gmin=-0.05)
+    v[0, cu[1] + 8000, 0, 5] = float("nan")
+    v[0, cu[3] + 1000, 1, 127] = float("inf")
+    k[0, cu[4] + 299, 0, 0] = float("nan")
+    g[0, cu[3] - 1, 0] = float("-inf")
+    pool = torch.randn(8, Hv, dk, dv, generator=torch.Generator().manual_seed(78))
+    index = torch.tensor([7, 0, 3, 5, 1, 2], dtype=torch.int32)
+    st = pool.to(DEV)
+    o, _ = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), st, scale=0.1, index=index.to(DEV), check=True,
+                           cu_seqlens=torch.tensor(cu, dtype=torch.int32, device=DEV))
+    o, fin = o.cpu(), st.cpu()
+    for n, (a, b) in enumerate(zip(cu[:-1], cu[1:])):
+        p = int(index[n])
+        if a == b:
+            assert torch.equal(fin[p], pool[p])
+            continue
+        ref = steps(q[0, a:b], k[0, a:b], v[0, a:b], g[0, a:b], pool[p], 0.1)
+        check_finite_part(o[0, a:b], fin[p], ref, io, k[0, a:b], v[0, a:b])
+    assert torch.equal(fin[[4, 6]], pool[[4, 6]])
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+def test_prefill_captured_and_on_two_streams(pkg, io):
+    """Replays on new inputs, and two calls in flight, give what single calls do, to the bit."""
+    sets = [[x.to(DEV) for x in make((2, 300), 1, 2, 128, 128, io, s)] for s in (79, 80)]
+    want = [pkg.lin_prefill(*x, check=True) for x in sets]
+    x = [t.clone() for t in sets[0]]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, S = pkg.lin_prefill(*x)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for i in (1, 0):
+        for a, b in zip(x, sets[i]):
+            a.copy_(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        got = []
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(pkg.lin_prefill(*sets[j]))
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[i][0]) and torch.equal(S, want[i][1])
+        assert all(torch.equal(a, b) for g1, w in zip(got, want) for a, b in zip(g1, w))
+    pkg.check_device_status(torch.device(DEV))
