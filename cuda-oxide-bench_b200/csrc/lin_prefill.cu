@@ -89,7 +89,7 @@ constexpr int kRanked = 64;
 constexpr float kLowest = -160.f;
 // How a chunk's decays are factored, by the range of G (in powers of two):
 //   kNear       G stays between -kLeast and kMost: e^(G_i) e^(-G_j)
-//   kNearBlock  no gate grows, and each block of 32 tokens spans at most kSpan:
+//   kNearBlock  no gate grows or resets, and each block of 32 tokens spans at most kSpan:
 //               e^(G_i - R_b) e^(R_b - G_j), R_b G at the end of j's block (where the
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
@@ -1036,9 +1036,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, off));
           hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, off));
         }
-        // (a NaN, which R_b would bring to the earlier rows of its block, fails this)
-        const bool falls = x[0] <= 0.f && x[1] <= 0.f && x[2] <= 0.f && x[3] <= 0.f;
-        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kSpan && falls);
+        // (a NaN, which R_b would bring to the earlier rows of its block, fails this; a decay of
+        // zero too: behind it nothing of the state may be left, not 2^-kLeast of it either)
+        const auto falls = [](float x) { return x <= 0.f && x > kLowest; };
+        const bool near_block = __all_sync(0xffffffffu, hi - lo <= kSpan && falls(x[0]) && falls(x[1]) && falls(x[2]) && falls(x[3]));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 8));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 8));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 16));

@@ -192,7 +192,7 @@ def lin_prefill(q, k, v, g, initial_state=None, *, scale: float = 1.0, cu_seqlen
     finite.  bf16: the decayed scores, and the state where the queries meet it, are
     rounded to bf16 once, the state itself takes its terms in 16 bits; under strong
     decay outputs hold up to 2^47, and a row keeps 2^-80 of the state before its chunk
-    (128 tokens) where the decay would leave less.  f16: scores rounded to f16 times a
+    (128 tokens) where the decay would leave less, but none behind a decay of zero.  f16: scores rounded to f16 times a
     power of two of their row, the state where the queries meet it to tf32, its terms
     in 22 bits; scores and states may pass f16's range (about twice the time of bf16).
     """

@@ -932,3 +932,16 @@ def test_prefill_captured_and_on_two_streams(pkg, io):
         assert torch.equal(o, want[i][0]) and torch.equal(S, want[i][1])
         assert all(torch.equal(a, b) for g1, w in zip(got, want) for a, b in zip(g1, w))
     pkg.check_device_status(torch.device(DEV))
+
+
+@pytest.mark.parametrize("io", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("at", [0, 64, 96, 128])
+def test_prefill_reset_drops_a_state_of_any_size(pkg, at, io):
+    """A page that holds whatever was there before, and a decay of zero at the start of a chunk or of a block in it."""
+    T, d = 200, 64
+    q, k, v, g = make((1, T), 1, 2, d, d, io, 81, gmin=-0.1)
+    g[0, at] = float("-inf")
+    S0 = torch.randn(1, 2, d, d, generator=torch.Generator().manual_seed(82)) * 1e30
+    o, S = pkg.lin_prefill(*(x.to(DEV) for x in (q, k, v, g)), S0.to(DEV), check=True)
+    ro, rS, oa, Sa = steps(q[0], k[0], v[0], g[0], S0[0], 1.0)
+    check_prefill(o[0, at:].cpu(), S[0].cpu(), (ro[at:], rS, oa[at:], Sa), io, k[0], v[0])
