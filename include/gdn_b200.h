@@ -430,9 +430,10 @@ int lin_decode_launch(const lin_decode_args_t* args, gdn_stream_t stream);
  * scores, and the state where the queries meet it, are rounded to bf16 once; the
  * state itself takes its terms in 16 bits and sums in fp32; outputs hold up to
  * 2^47, and a row takes 2^-80 of the state before its 128-token chunk where the
- * decay would leave less (none of it behind a decay of zero).  f16 I/O: the decayed scores are rounded to f16 times a
- * power of two of their row, the state where the queries meet it to tf32; the
- * state itself takes its terms in 22 bits; scores and states may pass f16's range.
+ * decay would leave less (none of it behind a decay of zero).  f16 I/O: the
+ * decayed scores are rounded to f16 times a power of two of their row, the state
+ * where the queries meet it to tf32; the state itself takes its terms in 22
+ * bits; scores and states may pass f16's range.
  */
 typedef struct {
   const void* q;              /* [B, T, Hqk, d_k] or packed [T, Hqk, d_k]    */
