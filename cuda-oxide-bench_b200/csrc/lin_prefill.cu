@@ -94,9 +94,10 @@ constexpr float kLowest = -160.f;
 //               first of the two is zero so is P)
 //   kFar        else, as across a reset: e^(G_i - G_j) by itself
 // In bf16 O is summed without its rows' factors, which are 2^-kLeast at least, but with the
-// scale's power of two (2^pow, |pow| <= 32): fp32 holds outputs of up to 2^47 then, and a row that decay leaves less of the state before the
-// chunk takes 2^-80 of it.  The state itself is taken as it is: scaled by a factor in
-// the middle of the range it would leave bf16 below, from 2^-46 on.
+// scale's power of two (2^pow, |pow| <= 32): fp32 holds outputs of up to 2^47 then, and a
+// row that decay leaves less of the state before the chunk takes 2^-80 of it.  The state
+// itself is taken as it is: times a factor in the middle of the range, which may be 2^-80,
+// it would leave bf16 from 2^-46 on.
 constexpr float kSpan = 100.f;
 constexpr float kLeast = 80.f, kMost = 40.f;
 enum { kNear = 0, kNearBlock = 1, kFar = 2 };
